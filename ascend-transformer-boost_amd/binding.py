@@ -226,6 +226,16 @@ class AtbmiPaInt8QCall(ctypes.Structure):
                                        "vDescale", "pScale", "mask", "out")] + [("maskRowByQuery", ctypes.c_int32)]
 
 
+class AtbmiPaInt4Call(ctypes.Structure):
+    """One atbmi_pa_int4_decode call (include/atbmi_kernels.h)."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "numHeads", "numKvHeads", "headDim", "blockSize", "numBlocks",
+                                              "maxBlocksPerSeq", "batch", "queryTokens", "maskLen")] + [
+        ("qkScale", ctypes.c_float), ("reserved", ctypes.c_int32)] + [
+        (n, ctypes.c_int64) for n in ("maskSeqStride", "maskHeadStride", "maskRowStride")] + [
+        (n, ctypes.c_void_p) for n in ("query", "keyCache", "valueCache", "keyParams", "valueParams", "blockTables",
+                                       "contextLens", "mask", "out")]
+
+
 class AtbmiMlaMaskFreeCall(ctypes.Structure):
     """One atbmi_mla_mask_free_expand call (include/atbmi_kernels.h)."""
     _fields_ = [("batch", ctypes.c_int32), ("numQueryRows", ctypes.c_int32), ("templateBatch", ctypes.c_int32),
@@ -295,6 +305,14 @@ def kernels():
         lib.atbmi_mla_int8_decode.argtypes = [ctypes.POINTER(AtbmiMlaInt8Call), vp, u64, vp]
         lib.atbmi_pa_int8q_workspace_size.argtypes = [ctypes.POINTER(AtbmiPaInt8QCall), ctypes.POINTER(u64)]
         lib.atbmi_pa_int8q_decode.argtypes = [ctypes.POINTER(AtbmiPaInt8QCall), vp, u64, vp]
+        lib.atbmi_rms_norm_quant.argtypes = [vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i32, ctypes.c_float, vp]
+        lib.atbmi_linear_int8_workspace_size.argtypes = [i64, i64, i64, ctypes.POINTER(u64)]
+        lib.atbmi_linear_int8.argtypes = [vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i32, vp, u64, vp]
+        lib.atbmi_reshape_and_cache_int4.argtypes = [vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i64, i32, vp]
+        lib.atbmi_paged_cache_load_int4.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i64,
+                                                    i64, i32, vp]
+        lib.atbmi_pa_int4_workspace_size.argtypes = [ctypes.POINTER(AtbmiPaInt4Call), ctypes.POINTER(u64)]
+        lib.atbmi_pa_int4_decode.argtypes = [ctypes.POINTER(AtbmiPaInt4Call), vp, u64, vp]
         lib.atbmi_pa_plan_destroy.argtypes = [vp]
         lib.atbmi_pa_plan_destroy.restype = None
         lib.atbmi_timing_enable.argtypes = [i32]

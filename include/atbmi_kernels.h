@@ -645,6 +645,131 @@ int atbmi_mla_mask_free_expand(const AtbmiMlaMaskFreeCall *call, void *workspace
                                void *stream);
 
 /*
+ * ---- Quantised decoder layer: 8-bit activations and weights, a cache in 4 bits ----
+ *
+ * No counterpart in the reference in this form. Five operators that make up the attention half of a decoder layer:
+ * atbmi_rms_norm_quant -> atbmi_linear_int8 -> atbmi_reshape_and_cache_int4 -> atbmi_pa_int4_decode ->
+ * atbmi_linear_int8, and atbmi_paged_cache_load_int4 for steps that need cached rows as plain tensors. Nothing is
+ * read from the host during a call (lengths, slots and tables are device memory) and nothing is allocated, copied or
+ * waited for, so every one of them can be captured into a HIP graph. The stream must belong to the current device.
+ */
+
+/*
+ * RMS norm with the residual's addition and an 8-bit output with one scale per row. For row i:
+ *   s = x[i] + residual[i] rounded to dtype (residual NULL: s = x[i]), stored to residualOut[i] unless that is NULL
+ *   y = s * gamma / sqrt(mean(s^2) + epsilon)          (fp32, not rounded in between)
+ *   scale[i] = max|y| / 127,  out[i] = rint(y / scale[i]) in [-127, 127]     (ties to even; max|y| = 0: scale 0, codes 0)
+ * A row with a value (or gamma with one) that is not finite gets scale NaN and codes 0; one whose products s * gamma all
+ * lie below 2^-118 counts as zeros. x and residual have row strides of their own
+ * (elements, >= dim); out and residualOut are [rows, dim] without gaps. residualOut may be x or residual itself
+ * when that has no gaps either. dtype (fp16 or bf16) is the type of x, residual, gamma and residualOut; dim <= 65536.
+ */
+int atbmi_rms_norm_quant(const void *xDevice, const void *residualDevice, const void *gammaDevice, int8_t *outDevice,
+                         float *scaleDevice, void *residualOutDevice, int64_t rows, int64_t dim, int64_t xRowStride,
+                         int64_t residualRowStride, int32_t dtype, float epsilon, void *stream);
+
+/*
+ * Product of 8-bit integers with a scale for each token and each output channel:
+ *   out[i][j] = xScale[i] * wScale[j] * sum_k x[i][k] * w[j][k] + bias[j]
+ * x int8 [m, k], w int8 [n, k], xScale fp32 [m], wScale fp32 [n], bias fp32 [n] or NULL, out fp16 / bf16 [m, n], each
+ * matrix with a row stride of its own (elements). The integer sum is exact (k <= 131071 keeps it within 32 bits); it is
+ * scaled in fp32 and rounded once. out may not overlap an input.
+ * The workspace (atbmi_linear_int8_workspace_size; its size follows the number of CUs of the current device, so size
+ * and launch belong on the same device) holds integer partial sums where the contraction is split; it needs no
+ * initial content. Size 0: workspaceDevice may be NULL.
+ */
+int atbmi_linear_int8_workspace_size(int64_t m, int64_t n, int64_t k, uint64_t *bytes);
+int atbmi_linear_int8(const int8_t *xDevice, const int8_t *wDevice, const float *xScaleDevice, const float *wScaleDevice,
+                      const float *biasDevice, void *outDevice, int64_t m, int64_t n, int64_t k, int64_t xRowStride,
+                      int64_t wRowStride, int64_t outRowStride, int32_t outDtype, void *workspaceDevice,
+                      uint64_t workspaceBytes, void *stream);
+
+/*
+ * The 4-bit cache. A row (token, KV head) of D channels is held as D codes of 4 bits and two 16-bit numbers, scale and
+ * middle, in the model's type; channel c stands for middle + (code[c] - 7.5) * scale:
+ *   keyCache    uint8  [numBlocks, numKvHeads, blockSize, D / 2]   byte i of a row: channels 2 i (low half) and 2 i + 1
+ *   valueCache  uint8  [numBlocks, numKvHeads, D / 2, blockSize]   byte (i, t): channels 2 i and 2 i + 1 of token t
+ *   keyParams, valueParams  dtype [numBlocks, numKvHeads, blockSize, 2]   (scale, middle)
+ * The value codes of a block lie channel after channel because the attention contracts over tokens. D is 64, 128 or
+ * 256, blockSize a multiple of 16 up to 1024; all four start on 16-byte boundaries. A block of each of the four is
+ * contiguous, so atbmi_block_copy moves it (two calls: codes, params).
+ */
+
+/*
+ * Writes one key and one value row per token: quantises it over its D channels and stores it in slot
+ * s = slotMapping[i] (block s / blockSize, place s % blockSize); a slot outside [0, numBlocks * blockSize) skips the
+ * token. With hi and lo the largest and smallest value of the row, scale = (hi - lo) / 15 and middle = (hi + lo) / 2,
+ * rounded to dtype, and code = rint((x - middle) / scale + 7.5) in [0, 15] (scale 0: code 8, so the row stands for its
+ * middle). A row with a value that is not finite gets scale and middle NaN. key and value are [numTokens, numKvHeads,
+ * D] with a token stride of their own (elements, >= numKvHeads * D): slices of a fused projection's output need no
+ * copy. The slots of one call must differ: of a slot named twice the content is undefined.
+ */
+int atbmi_reshape_and_cache_int4(const void *keyDevice, const void *valueDevice, uint8_t *keyCacheDevice,
+                                 uint8_t *valueCacheDevice, void *keyParamsDevice, void *valueParamsDevice,
+                                 const int32_t *slotMappingDevice, int64_t numTokens, int64_t numKvHeads, int64_t headDim,
+                                 int64_t blockSize, int64_t numBlocks, int64_t keyTokenStride, int64_t valueTokenStride,
+                                 int32_t dtype, void *stream);
+
+/*
+ * The reverse: token t of sequence b, t < seqLens[b], is the cached row at position p = seqStarts[b] + t of the
+ * sequence (seqStarts NULL: 0; a position of its own, not a block's), found in block blockTables[b][p / blockSize],
+ * and lands in row (tokens of the sequences before b) + t of key and value, dtype [outRows, numKvHeads, D] without
+ * gaps, 16-byte aligned. Left untouched: rows of positions outside the table or in blocks outside [0, numBlocks), and
+ * what lies at or past outRows. A length below zero counts as zero. maxSeqLen bounds the lengths (the launch is sized
+ * by it): tokens at or past it stay unread, but keep their rows.
+ */
+int atbmi_paged_cache_load_int4(const uint8_t *keyCacheDevice, const uint8_t *valueCacheDevice, const void *keyParamsDevice,
+                                const void *valueParamsDevice, const int32_t *blockTablesDevice,
+                                const int32_t *seqLensDevice, const int32_t *seqStartsDevice, void *keyDevice,
+                                void *valueDevice, int64_t batch, int64_t maxBlocksPerSeq, int64_t numKvHeads,
+                                int64_t headDim, int64_t blockSize, int64_t numBlocks, int64_t outRows, int64_t maxSeqLen,
+                                int32_t dtype, void *stream);
+
+/*
+ * Decode attention over the 4-bit cache, queryTokens consecutive query rows per sequence:
+ *   query, out  dtype [batch * queryTokens, numHeads, headDim]      blockTables int32 [batch, maxBlocksPerSeq]
+ *   contextLens int32 [batch], device memory                        query head h reads KV head h / (numHeads / numKvHeads)
+ * The last queryTokens positions of a context are the query tokens' own: the j-th sees the positions
+ * p < contextLens[b] - queryTokens + 1 + j. A length below 0 counts as 0, one past the table's reach as that reach.
+ * Positions in blocks outside [0, numBlocks) are not seen. With a mask (dtype), mask[b * maskSeqStride + h *
+ * maskHeadStride + j * maskRowStride + p] (elements; 0: shared) is added to the scaled score; -inf hides the position
+ * whatever its score is, and positions at or past maskLen are hidden too. A row that sees nothing is written as zeros.
+ * query and out start on 16-byte boundaries.
+ */
+typedef struct AtbmiPaInt4Call {
+    int32_t dtype;             /* ATBMI_F16 or ATBMI_BF16: query, mask, params and out */
+    int32_t numHeads;
+    int32_t numKvHeads;        /* divides numHeads */
+    int32_t headDim;           /* 64, 128 or 256 */
+    int32_t blockSize;         /* multiple of 16, at most 1024 */
+    int32_t numBlocks;
+    int32_t maxBlocksPerSeq;   /* maxBlocksPerSeq * blockSize < 2^30 */
+    int32_t batch;
+    int32_t queryTokens;       /* 1 .. 64 */
+    int32_t maskLen;           /* positions of a mask row; read only with a mask */
+    float qkScale;
+    int32_t reserved;          /* 0 */
+    int64_t maskSeqStride;
+    int64_t maskHeadStride;
+    int64_t maskRowStride;
+    const void *query;
+    const uint8_t *keyCache;
+    const uint8_t *valueCache;
+    const void *keyParams;
+    const void *valueParams;
+    const int32_t *blockTables;
+    const int32_t *contextLens;
+    const void *mask;          /* NULL: none */
+    void *out;
+} AtbmiPaInt4Call;
+
+/* Validates the call (pointers aside) and reports the device workspace it needs: partial rows of contexts that are
+ * worked on by several workgroups. It needs no initial content and is free again when the call's kernels are done;
+ * calls that may overlap need one each. Follows the number of CUs of the current device. */
+int atbmi_pa_int4_workspace_size(const AtbmiPaInt4Call *call, uint64_t *bytes);
+int atbmi_pa_int4_decode(const AtbmiPaInt4Call *call, void *workspaceDevice, uint64_t workspaceBytes, void *stream);
+
+/*
  * Kernel timing for benchmarks. atbmi_timing_enable(n) with n > 0 makes every
  * n-th atbmi_pa_decode bracket its attention kernel with HIP events on the
  * launch stream (the events themselves cost a few microseconds of stream
