@@ -28,6 +28,7 @@ template <bool BF16> __device__ __forceinline__ float MidOf(uint32_t word)
 
 struct RowParams {
     float inv; // 1 / scale, 0 where the scale is 0
+    float scale;
     float mid;
     uint32_t word;
 };
@@ -49,15 +50,21 @@ template <bool BF16> __device__ __forceinline__ RowParams ParamsOf(float hi, flo
     }
     const float s = Widen<BF16>(scale);
     p.inv = (bad || s == 0.0f) ? 0.0f : 1.0f / s;
+    p.scale = s;
     p.mid = bad ? 0.0f : Widen<BF16>(mid);
     p.word = static_cast<uint32_t>(scale) | (static_cast<uint32_t>(mid) << 16);
     return p;
 }
 
-// rint((x - mid) / scale + 7.5) in 0 .. 15; 8 where the scale is 0 or the row is not finite (x is then ignored).
+// rint((x - mid) / scale + 7.5) in 0 .. 15; 8 where the scale is 0 or the row is not finite (x is then ignored). All
+// three numbers have few bits, so whole quotients, which the half makes ties, are common: the product with 1 / scale is
+// corrected by its remainder, which makes them exact, and ties go to the even code as the definition has it.
 __device__ __forceinline__ uint32_t CodeOf(float x, const RowParams &p)
 {
-    const float q = p.inv == 0.0f ? 8.0f : rintf(__builtin_fmaf(x - p.mid, p.inv, 7.5f));
+    const float d = x - p.mid;
+    const float q0 = d * p.inv;
+    const float quotient = __builtin_fmaf(__builtin_fmaf(-q0, p.scale, d), p.inv, q0);
+    const float q = p.inv == 0.0f ? 8.0f : rintf(quotient + 7.5f);
     return static_cast<uint32_t>(fminf(fmaxf(q, 0.0f), 15.0f));
 }
 

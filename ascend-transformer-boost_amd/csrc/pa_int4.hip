@@ -5,10 +5,12 @@
 //   q . k_t   = ks_t (q . u_t - 7.5 sum q) + km_t sum q
 //   sum w v   = sum_t (w_t vs_t) (u_t - 7.5) + sum_t w_t vm_t
 // and both contractions run on the codes themselves: the scales meet the scores and the weights, one number a token
-// instead of one a channel. Codes become operands of the matrix instructions with one or two integer operations for
-// two of them: 0x4300 | u is the bf16 number 128 + u, and u alone is the fp16 number u 2^-24, both exact; the
-// constants (135.5 sum q; 135.5 sum of the rounded weights) are taken off in fp32 afterwards, against sums of exactly
-// the values that were multiplied.
+// instead of one a channel. Codes become operands of the matrix instructions with a shift and an and-or for two of
+// them: 0x4180 | u << 3 is the bf16 number 16 + u, and u alone is the fp16 number u 2^-24, both exact; the constants
+// (23.5 sum q; 23.5 sum of the rounded weights) are taken off in fp32 afterwards, against sums of exactly the values
+// that were multiplied. (0x4300 | u = 128 + u needs a shift less in eight values, but a long context's output is a
+// small difference of sums that carry the offset: at 5000 tokens of fp16 the error against 64 bits was 3.3e-4 with 128,
+// of which 2.1e-4 are the output's own rounding.)
 //
 // Layout of v_mfma_f32_16x16x32_{bf16,f16}: lane (c = lane % 16, kg = lane / 16) supplies contraction values 8 kg ..
 // 8 kg + 7 of row c (A) / column c (B) and receives D[4 kg + e][c], e = 0 .. 3. The order of the contraction is free as
@@ -131,9 +133,13 @@ template <bool BF16> __device__ __forceinline__ f32x4 Mfma(u32x4 a, u32x4 b, f32
 // Nibbles x and x + 4 (x = 0 .. 3) of a word as four operand registers.
 template <bool BF16> __device__ __forceinline__ u32x4 Spread(uint32_t w)
 {
-    constexpr uint32_t M = 0x000f000fu;
-    constexpr uint32_t ONE = BF16 ? 0x43004300u : 0u;
-    return u32x4{(w & M) | ONE, ((w >> 4) & M) | ONE, ((w >> 8) & M) | ONE, ((w >> 12) & M) | ONE};
+    if constexpr (BF16) {
+        constexpr uint32_t M = 0x00780078u, ONE = 0x41804180u;
+        return u32x4{((w << 3) & M) | ONE, ((w >> 1) & M) | ONE, ((w >> 5) & M) | ONE, ((w >> 9) & M) | ONE};
+    } else {
+        constexpr uint32_t M = 0x000f000fu;
+        return u32x4{w & M, (w >> 4) & M, (w >> 8) & M, (w >> 12) & M};
+    }
 }
 
 __device__ __forceinline__ uint32_t PackBf16(float a, float b)
@@ -149,8 +155,8 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
     constexpr int KW = D / 32; // 32-bit words of a token's codes a lane holds = matrix instructions a 16-token block
     constexpr int CT = D / 32; // tiles of 16 channel pairs
     constexpr int PITCH = D + 4;
-    // what 0x4300 | u and u stand for beyond u - 7.5, and the factor of u
-    constexpr float K_OFFSET = BF16 ? 135.5f : 7.5f;
+    // what the operands stand for beyond u - 7.5, and the factor of u
+    constexpr float K_OFFSET = BF16 ? 23.5f : 7.5f;
     constexpr float K_FACTOR = BF16 ? 1.0f : 16777216.0f;
     __shared__ float ldsO[PA_WAVES][HT][PITCH];
     __shared__ float ldsM[PA_WAVES][HT];
@@ -364,9 +370,9 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
 #pragma unroll
                 for (int i = 0; i < CT; ++i) {
                     const uint32_t w0 = vw[i][2 * h], w1 = vw[i][2 * h + 1];
-                    constexpr uint32_t M = 0x000f000fu, K = 0x43004300u;
-                    const u32x4 even = {(w0 & M) | K, ((w0 >> 8) & M) | K, (w1 & M) | K, ((w1 >> 8) & M) | K};
-                    const u32x4 odd = {((w0 >> 4) & M) | K, ((w0 >> 12) & M) | K, ((w1 >> 4) & M) | K, ((w1 >> 12) & M) | K};
+                    const u32x4 a0 = Spread<true>(w0), a1 = Spread<true>(w1); // low, high half of tokens 0, 2; of 1, 3
+                    const u32x4 even = {a0[0], a0[2], a1[0], a1[2]};
+                    const u32x4 odd = {a0[1], a0[3], a1[1], a1[3]};
                     acc[i][0] = Mfma<true>(even, pw, acc[i][0]);
                     acc[i][1] = Mfma<true>(odd, pw, acc[i][1]);
                     if constexpr (!BF16) {
@@ -395,7 +401,7 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
             if (kg == 0) {
                 ldsL[wave][c] = total * f;
             }
-            const float rest = mids - 135.5f * ones[0];
+            const float rest = mids - 23.5f * ones[0];
 #pragma unroll
             for (int i = 0; i < CT; ++i) {
                 float *to = &ldsO[wave][c][32 * i + 8 * kg];

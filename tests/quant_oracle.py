@@ -34,7 +34,7 @@ def attention(query, cache, tables, lens, qk_scale, tokens, block_size, mask=Non
     """(output, bound) float64 [batch * tokens, H, D] of paged_attention_int4, position by position of its definition.
 
     The bound counts: the output's rounding (U); the weights' rounding to bf16 (2^-8 of what they multiply, or 2^-16 for
-    fp16 models, which keep the remainder), the fp32 sums over codes offset by 135.5, and the scores' fp32 errors, which
+    fp16 models, which keep the remainder), the fp32 sums over codes offset by 23.5, and the scores' fp32 errors, which
     change a weight by their size."""
     dtype = query.dtype
     q = query.cpu().double()
@@ -79,9 +79,9 @@ def attention(query, cache, tables, lens, qk_scale, tokens, block_size, mask=Non
                 live = ~hide
                 o = (w[live, None] * v[live, kv]).sum(0)
                 out[b * tokens + j, head] = o
-                # fp32 in a score: sums of D terms (offset codes up to 150 times the scale, the middle), then a few more
+                # fp32 in a score: sums of D terms (offset codes up to 40 times the scale, the middle), then a few more
                 sum_q = q[b * tokens + j, head].abs().sum()
-                err = F32 * (2 * (d + 8) * (150.0 * ks[live, kv] + km[live, kv].abs()) * sum_q * qk_scale)
+                err = F32 * (2 * (d + 8) * (40.0 * ks[live, kv] + km[live, kv].abs()) * sum_q * qk_scale)
                 # (a mask of the type's lowest value leaves scores that differ by less than their last bit: no error in
                 # the differences that the weights are made of; the weights of others beside such scores are 0)
                 size = torch.where(s[live].abs() < 1e30, s[live].abs(), 0.0)
@@ -89,7 +89,7 @@ def attention(query, cache, tables, lens, qk_scale, tokens, block_size, mask=Non
                 vl, wl = v[live, kv], w[live]
                 spread = (wl[:, None] * (vl - vm[live, kv][:, None]).abs()).sum(0)
                 p_err = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -16
-                sums = F32 * (n / 32 + 96) * ((wl * vs[live, kv]).sum() * 150.0 + (wl * vm[live, kv].abs()).sum())
+                sums = F32 * (n / 32 + 96) * ((wl * vs[live, kv]).sum() * 40.0 + (wl * vm[live, kv].abs()).sum())
                 bound[b * tokens + j, head] = (U[dtype] * o.abs() + p_err * spread + 2 * err * (wl[:, None] * vl.abs()).sum(0) +
                                                sums + TINY[dtype]) * 1.01
     return out, bound
@@ -111,7 +111,9 @@ def quantised_row_ok(x, codes, params):
     c = torch.empty(v.shape, dtype=torch.float64)
     c[..., 0::2], c[..., 1::2] = (codes & 15).double(), (codes >> 4).double()
     place = ((v - mid[..., None]) / scale.clamp_min(1e-300)[..., None] + 7.5).clamp(0, 15)
-    near = ((c - place).abs() <= 0.5 + 64 * F32 * 16).all(-1)  # fp32: the difference, the reciprocal, the sum
+    near = (c - place).abs() <= 0.5 + 64 * F32 * 16  # fp32: the difference, the reciprocal, the sum
+    tie = (place - place.floor() == 0.5) & ((v - mid[..., None]).float().double() == v - mid[..., None])
+    near = (near & (~tie | (c == place.round()))).all(-1)  # exact ties, common with so few bits, go to the even code
     good &= torch.where(scale == 0, (c == 8).all(-1), near)
     return bool((ok | (finite & good)).all())
 
