@@ -32,13 +32,19 @@ __device__ __forceinline__ uint16_t Rounded(const Args &a, float v)
     return a.bf16 ? FloatToBf16(v) : FloatToHalfBits(v);
 }
 
-// Sixteen values from an address of any alignment; those at or past `valid` count as zero.
-__device__ __forceinline__ i32x4 Load16Any(const int8_t *p, int valid)
+// Sixteen values from an address of any alignment, those at or past `valid` zero; the row they end is `row` values long.
+// Where the row ends inside them (or in front of them) its last sixteen are read instead and shifted, so that every lane
+// makes one load and no branch stands between the loads of a stage.
+__device__ __forceinline__ i32x4 Load16Any(const int8_t *p, int valid, int row)
 {
     i32x4 v = {0, 0, 0, 0};
-    if (valid >= 16) {
-        __builtin_memcpy(&v, p, 16);
-    } else if (valid > 0) {
+    if (row >= 16) { // (the same for all)
+        const int missing = min(max(16 - valid, 0), 16);
+        unsigned __int128 wide;
+        __builtin_memcpy(&wide, p + min(valid - 16, 0), 16);
+        wide = missing < 16 ? wide >> (8 * missing) : 0;
+        __builtin_memcpy(&v, &wide, 16);
+    } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int byte = i < valid ? static_cast<uint8_t>(p[i]) : 0;
@@ -288,7 +294,7 @@ __global__ __launch_bounds__(ANY_WAVES *WAVE, 2) void LinearAnyKernel(const Args
         }
 #pragma unroll
         for (int i = 0; i < MOVES; ++i) {
-            held[i] = Load16Any((8 * ANY_WAVES * i < ANY_TILE ? wBase : xBase) + at[i] + k0, kEnd - k0 - chunk16);
+            held[i] = Load16Any((8 * ANY_WAVES * i < ANY_TILE ? wBase : xBase) + at[i] + k0, kEnd - k0 - chunk16, kEnd);
         }
     };
     auto arrive = [&](int buffer) {
@@ -418,7 +424,7 @@ __global__ __launch_bounds__(RING_WAVES *WAVE, 2) void LinearRingKernel(const Ar
 #pragma unroll
                 for (int i = 0; i < ROWS; ++i) {
                     *reinterpret_cast<i32x4 *>(lds + slot * STAGE + part * PART + (wave + RING_WAVES * i) * 1024 + lane * 16) =
-                        Load16Any(base[i] + k0 + 64 * part + at[i], kEnd - k0 - 64 * part - chunk16);
+                        Load16Any(base[i] + k0 + 64 * part + at[i], kEnd - k0 - 64 * part - chunk16, kEnd);
                 }
             }
         }
@@ -643,7 +649,7 @@ __global__ __launch_bounds__(SKINNY_WAVES *WAVE, 1) void LinearSkinnyKernel(cons
 #pragma unroll
         for (int i = 0; i < MOVES; ++i) {
             *reinterpret_cast<i32x4 *>(mine + i * 1024 + lane * 16) =
-                Load16Any((i < 2 * CT ? wBase : xBase) + k + at[i], kEnd - k - chunk16);
+                Load16Any((i < 2 * CT ? wBase : xBase) + k + at[i], kEnd - k - chunk16, kEnd);
         }
         WaveSync();
         fetch(0);
