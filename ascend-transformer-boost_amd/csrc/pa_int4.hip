@@ -47,6 +47,7 @@ constexpr int TW = 64;          // tokens a tile
 constexpr int HT = 16;          // columns a workgroup
 constexpr int PA_WAVES = 4;
 constexpr int PA_THREADS = PA_WAVES * WAVE;
+constexpr int MERGE_MOST_THREADS = 1024;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float STEP_UP = 8.0f; // how far (log2) a score may exceed the reference before that moves
 
@@ -67,6 +68,7 @@ struct PaInt4Args {
     int64_t maskHeadStride;
     int64_t maskRowStride;
     int32_t maskLen;
+    int32_t maskVec; // every mask row starts on a 16-byte boundary
     int32_t H;
     int32_t G;
     int32_t group; // H / G
@@ -97,7 +99,7 @@ __device__ __forceinline__ int WaveSum(int v)
     for (int step = 1; step < WAVE; step *= 2) {
         v += __shfl_xor(v, step);
     }
-    return v;
+    return __builtin_amdgcn_readfirstlane(v);
 }
 
 // Ranges that get work: none shorter than a tile for each wave.
@@ -134,12 +136,19 @@ template <bool BF16> __device__ __forceinline__ f32x4 Mfma(u32x4 a, u32x4 b, f32
 template <bool BF16> __device__ __forceinline__ u32x4 Spread(uint32_t w)
 {
     if constexpr (BF16) {
-        constexpr uint32_t M = 0x00780078u, ONE = 0x41804180u;
-        return u32x4{((w << 3) & M) | ONE, ((w >> 1) & M) | ONE, ((w >> 5) & M) | ONE, ((w >> 9) & M) | ONE};
+        // (one instruction for the and and the or wants its constants in registers: two literals would make two of it)
+        uint32_t m = 0x00780078u, one = 0x41804180u;
+        asm("" : "+s"(m), "+v"(one));
+        return u32x4{((w << 3) & m) | one, ((w >> 1) & m) | one, ((w >> 5) & m) | one, ((w >> 9) & m) | one};
     } else {
         constexpr uint32_t M = 0x000f000fu;
         return u32x4{w & M, (w >> 4) & M, (w >> 8) & M, (w >> 12) & M};
     }
+}
+
+__device__ __forceinline__ uint32_t LdsAddress(const void *p)
+{
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void *)p));
 }
 
 __device__ __forceinline__ uint32_t PackBf16(float a, float b)
@@ -149,16 +158,47 @@ __device__ __forceinline__ uint32_t PackBf16(float a, float b)
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
 }
 
+// 16 bytes (4 bytes) a lane from its address to LDS at ldsAt + 16 (4) x lane, read once: not to displace anything.
+__device__ __forceinline__ void ToLds16(const void *from, uint32_t ldsAt)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(ldsAt), "v"(from) : "memory", "m0");
+}
+__device__ __forceinline__ void ToLds4(const void *from, uint32_t ldsAt)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off nt" ::"s"(ldsAt), "v"(from) : "memory", "m0");
+}
+
+// A wave's tile in LDS: key codes token after token (rows of D / 2 bytes), value codes in blocks of 16 channel pairs by 64
+// tokens (rows of 64 bytes), the params of the 64 keys, those of the values. The 16-byte pieces of a row are permuted by an
+// exclusive or so that the rows the matrix instruction reads side by side lie in different banks.
+template <int D> struct TileLayout {
+    static constexpr int KEYS = TW * D / 2, VALUES = TW * D / 2;
+    static constexpr int PARAMS = KEYS + VALUES;
+    static constexpr int BYTES = PARAMS + 2 * TW * 4;
+    static constexpr int PIECES = D / 32; // 16-byte pieces of a key row
+    static constexpr int MOVES = 2 * (KEYS / 1024) + 2;
+    static constexpr int SLOTS = D == 64 ? 3 : 2; // tiles of a wave that are in LDS or on their way
+    // what the place of a piece is its index xor-ed with, for token `row` of 16-token group `grp`: the lanes of a read hold
+    // four neighbouring rows of four groups
+    static __device__ __forceinline__ int KeyTwist(int row, int grp)
+    {
+        return D == 64 ? (grp & 1) : (D == 128 ? ((row / 2 + grp) & 3) : ((row & 3) | ((grp & 1) << 2)));
+    }
+    static constexpr int JOIN = 16 * (D + 4) * 4; // a wave's sums at the end of a sequence
+    static_assert(JOIN <= SLOTS * BYTES, "the sums take the place of the tiles");
+};
+
 template <int D, bool BF16, bool MASK>
 __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(const PaInt4Args a)
 {
+    using L = TileLayout<D>;
     constexpr int KW = D / 32; // 32-bit words of a token's codes a lane holds = matrix instructions a 16-token block
     constexpr int CT = D / 32; // tiles of 16 channel pairs
     constexpr int PITCH = D + 4;
     // what the operands stand for beyond u - 7.5, and the factor of u
     constexpr float K_OFFSET = BF16 ? 23.5f : 7.5f;
     constexpr float K_FACTOR = BF16 ? 1.0f : 16777216.0f;
-    __shared__ float ldsO[PA_WAVES][HT][PITCH];
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[]; // a ring of tiles for each wave
     __shared__ float ldsM[PA_WAVES][HT];
     __shared__ float ldsL[PA_WAVES][HT];
 
@@ -210,13 +250,64 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
     const int qTok = col / a.group;
     const int qHead = g * a.group + col % a.group;
     const int liveCols = min(HT, columns - ct * HT);
+    unsigned char *mine = lds + wave * L::SLOTS * L::BYTES;
+    const uint32_t mineAt = LdsAddress(mine);
+    const uint32_t maskAt = LdsAddress(lds + PA_WAVES * L::SLOTS * L::BYTES + wave * 2048); // MASK only
 
     for (int at = begin; at < end;) {
         const int len = ContextLen(a, seq);
         const int seqTiles = TilesOf(len);
         const int tBegin = at - before;
         const int tEnd = min(seqTiles, end - before);
-        const int32_t *table = a.tables + static_cast<int64_t>(seq) * a.maxBlocksPerSeq;
+        // (read through the scalar cache: block ids are not counted with the tiles on their way)
+        const auto *table = reinterpret_cast<const __attribute__((address_space(4))) int32_t *>(
+            reinterpret_cast<uintptr_t>(a.tables + static_cast<int64_t>(seq) * a.maxBlocksPerSeq));
+
+        // ---- asks for tile t; returns which of its four 16-token groups lie in blocks that exist, as bits
+        auto request = [&](int t, int slot) {
+            const uint32_t to = mineAt + slot * L::BYTES;
+            uint32_t there = 0;
+            int64_t first[4]; // of a group: its block's head, counted in rows of blockSize tokens
+            int place[4];     // and its first token within the block
+#pragma unroll
+            for (int grp = 0; grp < 4; ++grp) {
+                const uint32_t x = static_cast<uint32_t>(t * (TW / 16) + grp);
+                const uint32_t at16 = a.groupsMagic ? static_cast<uint32_t>((static_cast<uint64_t>(x) * a.groupsMagic) >> 32) : x;
+                const int id = table[min(static_cast<int>(at16), a.maxBlocksPerSeq - 1)];
+                const bool ok = id >= 0 && id < a.numBlocks;
+                there |= ok ? 1u << grp : 0u;
+                first[grp] = static_cast<int64_t>(ok ? id : 0) * a.G + g;
+                place[grp] = static_cast<int>(x - at16 * a.groupsPerBlock) * 16;
+            }
+            auto headOf = [&](int grp) { // (a lane's own choice of four values of the wave)
+                const int64_t lo = grp == 0 ? first[0] : int64_t(first[1]), hi = grp == 2 ? first[2] : int64_t(first[3]);
+                return grp < 2 ? lo : int64_t(hi);
+            };
+            auto placeOf = [&](int grp) {
+                const int lo = grp == 0 ? place[0] : int(place[1]), hi = grp == 2 ? place[2] : int(place[3]);
+                return grp < 2 ? lo : int(hi);
+            };
+#pragma unroll
+            for (int i = 0; i < L::KEYS / 1024; ++i) {
+                constexpr int ROWS = 1024 / (D / 2); // tokens an instruction moves
+                const int token = ROWS * i + lane / L::PIECES;
+                const int grp = token / 16, row = token % 16;
+                const int piece = (lane % L::PIECES) ^ L::KeyTwist(row, grp);
+                const int64_t head = ROWS <= 16 ? first[ROWS * i / 16 % 4] : headOf(grp);
+                const int in = ROWS <= 16 ? place[ROWS * i / 16 % 4] : placeOf(grp);
+                ToLds16(a.kc + (head * a.blockSize + in + row) * (D / 2) + piece * 16, to + i * 1024);
+            }
+            const int vGrp = (lane % 4) ^ (lane / 8 % 4);
+            const uint8_t *v = a.vc + (headOf(vGrp) * (D / 2) + lane / 4) * a.blockSize + placeOf(vGrp);
+#pragma unroll
+            for (int i = 0; i < CT; ++i) {
+                ToLds16(v + static_cast<int64_t>(16 * i) * a.blockSize, to + L::KEYS + i * 1024);
+            }
+            const int64_t param = headOf(kg) * a.blockSize + placeOf(kg) + c;
+            ToLds4(a.kp + param, to + L::PARAMS);
+            ToLds4(a.vp + param, to + L::PARAMS + TW * 4);
+            return there;
+        };
 
         // ---- the query columns, permuted as Spread orders the codes, and their sums
         u32x4 q[KW];
@@ -250,59 +341,95 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
         float total = 0.0f;    // of the lane's own tokens
         float mids = 0.0f;
 
-        for (int t = tBegin + wave; t < tEnd; t += PA_WAVES) {
+        // Mask values of the lane's 16 tokens of a tile, two a word. Rows on 16-byte boundaries come through LDS, asked for a
+        // tile ahead; others, and those of the tile in which the mask ends, are read where they are used.
+        auto maskAhead = [&](int t) { return a.maskVec != 0 && (t + 1) * TW <= a.maskLen; };
+        auto requestMask = [&](int t) {
+            const uint16_t *m = maskRow + t * TW + 16 * kg;
+            ToLds16(m, maskAt);
+            ToLds16(m + 8, maskAt + 1024);
+        };
+        auto readMask = [&](int t, uint32_t (&m)[8]) {
+            if (maskAhead(t)) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const u32x4 w = *reinterpret_cast<const u32x4 *>(lds + PA_WAVES * L::SLOTS * L::BYTES + wave * 2048 + 1024 * i + 16 * lane);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        m[4 * i + e] = w[e];
+                    }
+                }
+            } else {
+                const int first = t * TW + 16 * kg;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t lo = maskRow[min(first + 2 * i, a.maskLen - 1)];
+                    const uint32_t hi = maskRow[min(first + 2 * i + 1, a.maskLen - 1)];
+                    m[i] = lo | (hi << 16);
+                }
+            }
+        };
+
+        uint32_t there[L::SLOTS];
+        if constexpr (MASK) {
+            if (tBegin + wave < tEnd && maskAhead(tBegin + wave)) {
+                requestMask(tBegin + wave);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < L::SLOTS; ++i) {
+            there[i] = 0;
+            const int t = tBegin + wave + i * PA_WAVES;
+            if (t < tEnd) {
+                there[i] = request(t, i);
+            }
+        }
+
+        // (HIDDEN: some token of the tile may be hidden from some column)
+        auto tile = [&](int t, int slot, uint32_t ok4, auto hidden) {
+            constexpr bool HIDDEN = MASK || decltype(hidden)::value;
             const int t0 = t * TW;
-            // ---- block of a 16-token group of the tile; `ok` is false where the id is none
-            auto blockOf = [&](int grp, int &place, bool &ok) {
-                const uint32_t x = static_cast<uint32_t>(t0 / 16 + grp);
-                const uint32_t at16 = a.groupsMagic ? __umulhi(x, a.groupsMagic) : x;
-                place = static_cast<int>(x - at16 * a.groupsPerBlock) * 16;
-                const int id = table[min(static_cast<int>(at16), a.maxBlocksPerSeq - 1)];
-                ok = id >= 0 && id < a.numBlocks;
-                return static_cast<int64_t>(ok ? id : 0) * a.G + g;
-            };
-            int kPlace, vPlace;
-            bool kOk, vOk;
-            const int64_t kHead = blockOf(c >> 2, kPlace, kOk);
-            const int64_t vHead = blockOf(kg, vPlace, vOk);
-            // ---- codes
-            uint32_t kw[4][KW];
-#pragma unroll
-            for (int st = 0; st < 4; ++st) {
-                const uint8_t *at8 = a.kc + (kHead * a.blockSize + kPlace + 4 * st + (c & 3)) * (D / 2) + kg * (D / 8);
-                __builtin_memcpy(kw[st], __builtin_assume_aligned(at8, D / 8 < 16 ? 8 : 16), D / 8);
-            }
-            u32x4 vw[CT];
-#pragma unroll
-            for (int i = 0; i < CT; ++i) {
-                vw[i] = *reinterpret_cast<const u32x4 *>(a.vc + (vHead * (D / 2) + 16 * i + c) * a.blockSize + vPlace);
-            }
-            u32x4 kpw[4], vpw[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                kpw[i] = reinterpret_cast<const u32x4 *>(a.kp + vHead * a.blockSize + vPlace)[i];
-                vpw[i] = reinterpret_cast<const u32x4 *>(a.vp + vHead * a.blockSize + vPlace)[i];
+            const unsigned char *from = mine + slot * L::BYTES;
+            const int first = t0 + 16 * kg;
+            uint32_t maskBits[8];
+            if constexpr (MASK) {
+                readMask(t, maskBits);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (t + PA_WAVES < tEnd && maskAhead(t + PA_WAVES)) {
+                    requestMask(t + PA_WAVES);
+                }
             }
             // ---- scores of tokens t0 + 16 kg + j, in log2 units
             float s[16];
 #pragma unroll
             for (int st = 0; st < 4; ++st) {
+                const int row = 4 * st + (c & 3), grp = c >> 2;
+                uint32_t kw[KW];
+                const unsigned char *kr = from + (16 * grp + row) * (D / 2);
+                const int twist = L::KeyTwist(row, grp);
+                if constexpr (D == 64) {
+                    __builtin_memcpy(kw, __builtin_assume_aligned(kr + ((kg / 2) ^ twist) * 16 + (kg % 2) * 8, 8), 8);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < D / 128; ++i) {
+                        __builtin_memcpy(kw + 4 * i, __builtin_assume_aligned(kr + ((D / 128 * kg + i) ^ twist) * 16, 16), 16);
+                    }
+                }
                 f32x4 dot = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int i = 0; i < KW; ++i) {
-                    dot = Mfma<BF16>(Spread<BF16>(kw[st][i]), q[i], dot);
+                    dot = Mfma<BF16>(Spread<BF16>(kw[i]), q[i], dot);
                 }
+                const u32x4 kpw = *reinterpret_cast<const u32x4 *>(from + L::PARAMS + 64 * kg + 16 * st);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint32_t word = kpw[st][e];
-                    s[4 * st + e] = __builtin_fmaf(ScaleOf<BF16>(word), __builtin_fmaf(dot[e], facQ, offQ), MidOf<BF16>(word) * midQ);
+                    s[4 * st + e] = __builtin_fmaf(ScaleOf<BF16>(kpw[e]), __builtin_fmaf(dot[e], facQ, offQ), MidOf<BF16>(kpw[e]) * midQ);
                 }
             }
-            const int first = t0 + 16 * kg;
             if constexpr (MASK) {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    const float m = Widen<BF16>(maskRow[min(first + j, a.maskLen - 1)]);
+                    const float m = Widen<BF16>(static_cast<uint16_t>(maskBits[j / 2] >> (16 * (j % 2))));
                     // (the lowest finite value leaves fp32 when it is turned into log2 units: it stays finite here, so that
                     // a row of nothing else is the mean of its values; NaN stays NaN)
                     float v = __builtin_fmaf(m, LOG2E, s[j]);
@@ -310,10 +437,11 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
                     s[j] = (m == -INFINITY || first + j >= a.maskLen) ? -INFINITY : v;
                 }
             }
-            if (t0 + TW > allSee || __ballot(!vOk) != 0) {
+            if constexpr (HIDDEN) {
+                const bool ok = ((ok4 >> kg) & 1) != 0;
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    s[j] = vOk && first + j < seen ? s[j] : -INFINITY;
+                    s[j] = ok && first + j < seen ? s[j] : -INFINITY;
                 }
             }
             // ---- weights
@@ -338,46 +466,80 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
             const float base = top == -INFINITY ? 0.0f : top;
             float pv[16];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float p = __builtin_amdgcn_exp2f(s[j] - base);
-                const uint32_t word = vpw[j / 4][j % 4];
-                total += p;
-                // (a hidden token's params may hold anything: 0 times them must be 0)
-                const bool none = s[j] == -INFINITY;
-                pv[j] = none ? 0.0f : p * ScaleOf<BF16>(word);
-                mids += none ? 0.0f : p * MidOf<BF16>(word);
+            for (int j4 = 0; j4 < 4; ++j4) {
+                const u32x4 vpw = *reinterpret_cast<const u32x4 *>(from + L::PARAMS + TW * 4 + 64 * kg + 16 * j4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int j = 4 * j4 + e;
+                    const float p = __builtin_amdgcn_exp2f(s[j] - base);
+                    total += p;
+                    // (a hidden token's params may hold anything: 0 times them must be 0)
+                    const uint32_t word = HIDDEN && s[j] == -INFINITY ? 0u : vpw[e];
+                    pv[j] = p * ScaleOf<BF16>(word);
+                    mids = __builtin_fmaf(p, MidOf<BF16>(word), mids);
+                }
             }
             // ---- values. The weights (times the value scale) are rounded to bf16, which has fp32's range whatever the
             // scales are: an error of at most 2^-8 each for bf16 models, whose output is rounded as coarsely; for fp16
             // models the remainder is multiplied as well (2^-16 left).
+            u32x4 pw[2], pr[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                u32x4 pw, pr;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int j = 8 * h + 4 * (e / 2) + e % 2; // tokens j and j + 2 share a register, as Spread leaves them
-                    pw[e] = PackBf16(pv[j], pv[j + 2]);
+                    pw[h][e] = PackBf16(pv[j], pv[j + 2]);
                     if constexpr (!BF16) {
-                        pr[e] = PackBf16(pv[j] - __uint_as_float(pw[e] << 16), pv[j + 2] - __uint_as_float(pw[e] & 0xffff0000u));
+                        pr[h][e] = PackBf16(pv[j] - __uint_as_float(pw[h][e] << 16), pv[j + 2] - __uint_as_float(pw[h][e] & 0xffff0000u));
                     }
                 }
                 constexpr uint32_t ONE = 0x3f803f80u;
                 const u32x4 one = {ONE, ONE, ONE, ONE};
-                ones = Mfma<true>(one, pw, ones);
+                ones = Mfma<true>(one, pw[h], ones);
                 if constexpr (!BF16) {
-                    ones = Mfma<true>(one, pr, ones);
+                    ones = Mfma<true>(one, pr[h], ones);
                 }
+            }
 #pragma unroll
-                for (int i = 0; i < CT; ++i) {
-                    const uint32_t w0 = vw[i][2 * h], w1 = vw[i][2 * h + 1];
-                    const u32x4 a0 = Spread<true>(w0), a1 = Spread<true>(w1); // low, high half of tokens 0, 2; of 1, 3
-                    const u32x4 even = {a0[0], a0[2], a1[0], a1[2]};
+            for (int i = 0; i < CT; ++i) {
+                const u32x4 vw = *reinterpret_cast<const u32x4 *>(from + L::KEYS + i * 1024 + c * 64 + 16 * (kg ^ (c / 2 % 4)));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const u32x4 a0 = Spread<true>(vw[2 * h]), a1 = Spread<true>(vw[2 * h + 1]);
+                    const u32x4 even = {a0[0], a0[2], a1[0], a1[2]}; // low half, then high half, of tokens 0, 2 and 1, 3
                     const u32x4 odd = {a0[1], a0[3], a1[1], a1[3]};
-                    acc[i][0] = Mfma<true>(even, pw, acc[i][0]);
-                    acc[i][1] = Mfma<true>(odd, pw, acc[i][1]);
+                    acc[i][0] = Mfma<true>(even, pw[h], acc[i][0]);
+                    acc[i][1] = Mfma<true>(odd, pw[h], acc[i][1]);
                     if constexpr (!BF16) {
-                        acc[i][0] = Mfma<true>(even, pr, acc[i][0]);
-                        acc[i][1] = Mfma<true>(odd, pr, acc[i][1]);
+                        acc[i][0] = Mfma<true>(even, pr[h], acc[i][0]);
+                        acc[i][1] = Mfma<true>(odd, pr[h], acc[i][1]);
+                    }
+                }
+            }
+        };
+
+        // ---- tiles. A slot is waited for by the number of loads that were asked for behind it (with a mask: behind the
+        // tile's mask values, which are asked for after all tiles but the last).
+        constexpr int BEHIND = MASK ? L::MOVES : (L::SLOTS - 1) * L::MOVES;
+        for (int t = tBegin + wave; t < tEnd; t += L::SLOTS * PA_WAVES) {
+#pragma unroll
+            for (int i = 0; i < L::SLOTS; ++i) {
+                const int now = t + i * PA_WAVES;
+                if (now < tEnd) {
+                    if (now + (L::SLOTS - 1) * PA_WAVES < tEnd) {
+                        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(BEHIND) : "memory");
+                    } else {
+                        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    }
+                    if (!MASK && (now + 1) * TW <= allSee && there[i] == 15u) {
+                        tile(now, i, 15u, std::false_type{});
+                    } else {
+                        tile(now, i, there[i], std::true_type{});
+                    }
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the slot has been read
+                    const int later = now + L::SLOTS * PA_WAVES;
+                    if (later < tEnd) {
+                        there[i] = request(later, i);
                     }
                 }
             }
@@ -387,7 +549,7 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
         total = QuadSum(total);
         mids = QuadSum(mids);
         const int busy = min(PA_WAVES, tEnd - tBegin);
-        __syncthreads(); // (the rows of the sequence before have been read)
+        auto sums = [&](int w) { return reinterpret_cast<float *>(lds + w * L::SLOTS * L::BYTES); }; // [16][PITCH]
         if (kg == 0) {
             ldsM[wave][c] = top;
         }
@@ -404,7 +566,7 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
             const float rest = mids - 23.5f * ones[0];
 #pragma unroll
             for (int i = 0; i < CT; ++i) {
-                float *to = &ldsO[wave][c][32 * i + 8 * kg];
+                float *to = sums(wave) + c * PITCH + 32 * i + 8 * kg;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     to[2 * e] = top == -INFINITY ? 0.0f : (acc[i][0][e] + rest) * f;
@@ -421,7 +583,7 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
             f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
             float l = 0.0f;
             for (int w = 0; w < busy; ++w) {
-                o += *reinterpret_cast<const f32x4 *>(&ldsO[w][n][d]);
+                o += *reinterpret_cast<const f32x4 *>(sums(w) + n * PITCH + d);
                 l += ldsL[w][n];
             }
             if (whole) {
@@ -449,14 +611,24 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
         before += seqTiles;
         at = before;
         ++seq;
+        if (at < end) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads(); // (the sums have been read: tiles may take their place)
+        }
     }
 }
 
 // Joins the parts of a sequence that was cut: out = sum 2^(M_p - M) O_p / sum 2^(M_p - M) L_p. A workgroup takes one
-// sequence and one pair; a thread four channels of a column.
-template <int D, bool BF16> __global__ __launch_bounds__(PA_THREADS) void PaInt4MergeKernel(const PaInt4Args a)
+// sequence and one pair. D / 4 lanes hold a column, four channels each, and look at that many parts at a time together for
+// the maxima and sums. Waves beyond those that the columns need share out the parts. (One sequence of 32768 tokens, 64
+// parts a head: 36 us when each thread walked all parts of its channels.)
+template <int D, bool BF16> __global__ __launch_bounds__(MERGE_MOST_THREADS) void PaInt4MergeKernel(const PaInt4Args a)
 {
+    constexpr int LANES = D / 4;          // lanes a column
+    constexpr int COLS = WAVE / LANES;    // columns a wave
+    __shared__ f32x4 shared[MERGE_MOST_THREADS];
     const int lane = threadIdx.x & (WAVE - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int pairs = a.G * a.colTiles;
     const int seq = blockIdx.x / pairs;
     const int pair = blockIdx.x % pairs;
@@ -476,37 +648,64 @@ template <int D, bool BF16> __global__ __launch_bounds__(PA_THREADS) void PaInt4
         return static_cast<int>(((static_cast<int64_t>(tile) + 1) * live - 1) / tiles);
     };
     const int r0 = rangeOf(before);
-    const int r1 = rangeOf(last);
-    if (r0 == r1) {
+    const int parts = rangeOf(last) - r0 + 1;
+    if (parts == 1) {
         return;
     }
-    const int columns = a.group * a.tokens;
-    const int liveCols = min(HT, columns - ct * HT);
+    const int liveCols = min(HT, a.group * a.tokens - ct * HT);
+    const int waves = blockDim.x / WAVE;
+    const int colWaves = min((liveCols + COLS - 1) / COLS, waves); // waves that the columns are spread over
+    const int slices = waves / colWaves;
+    const int slice = wave / colWaves;
+    const int q = lane % LANES;
     // (the part that begins the sequence is its range's second kind, the others are the first)
-    auto partOf = [&](int r) { return static_cast<int64_t>(2 * r + (r == r0 ? 1 : 0)) * pairs + pair; };
-    for (int i = threadIdx.x; i < liveCols * (D / 4); i += PA_THREADS) {
-        const int n = i / (D / 4);
-        const int d = i % (D / 4) * 4;
+    auto rowOf = [&](int p, int n) { return (static_cast<int64_t>(2 * (r0 + p) + (p == 0 ? 1 : 0)) * pairs + pair) * HT + n; };
+    for (int n0 = wave % colWaves * COLS; n0 < liveCols; n0 += colWaves * COLS) { // (as often for every slice)
+        const int n = min(n0 + lane / LANES, liveCols - 1);
         float top = -INFINITY;
-        for (int r = r0; r <= r1; ++r) {
-            top = fmaxf(top, a.partM[partOf(r) * HT + n]);
+        for (int p = q; p < parts; p += LANES) {
+            top = fmaxf(top, a.partM[rowOf(p, n)]);
+        }
+#pragma unroll
+        for (int step = 1; step < LANES; step *= 2) {
+            top = fmaxf(top, __shfl_xor(top, step));
+        }
+        auto weightOf = [&](int p) {
+            const float m = a.partM[rowOf(p, n)];
+            return m == -INFINITY ? 0.0f : exp2f(m - top);
+        };
+        float l = 0.0f;
+        for (int p = q; p < parts; p += LANES) {
+            l += weightOf(p) * a.partL[rowOf(p, n)];
+        }
+#pragma unroll
+        for (int step = 1; step < LANES; step *= 2) {
+            l += __shfl_xor(l, step);
         }
         f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-        float l = 0.0f;
-        for (int r = r0; r <= r1; ++r) {
-            const int64_t at = partOf(r) * HT + n;
-            const float m = a.partM[at];
-            const float w = m == -INFINITY ? 0.0f : exp2f(m - top);
-            l += w * a.partL[at];
-            o += w * *reinterpret_cast<const f32x4 *>(a.partO + at * D + d);
+        if (slice < slices) { // (waves that do not make up a whole slice hold nothing)
+#pragma unroll 4
+            for (int p = slice; p < parts; p += slices) {
+                o += weightOf(p) * *reinterpret_cast<const f32x4 *>(a.partO + rowOf(p, n) * D + 4 * q);
+            }
         }
-        const float inv = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l);
-        const int cc = ct * HT + n;
-        uint16_t *dst = a.out + ((static_cast<int64_t>(seq) * a.tokens + cc / a.group) * a.H + g * a.group + cc % a.group) * D + d;
-        u32x2 w;
-        w[0] = static_cast<uint32_t>(Narrow<BF16>(o[0] * inv)) | (static_cast<uint32_t>(Narrow<BF16>(o[1] * inv)) << 16);
-        w[1] = static_cast<uint32_t>(Narrow<BF16>(o[2] * inv)) | (static_cast<uint32_t>(Narrow<BF16>(o[3] * inv)) << 16);
-        *reinterpret_cast<u32x2 *>(dst) = w;
+        if (slices > 1) {
+            shared[threadIdx.x] = o;
+            __syncthreads();
+            for (int s = 1; s < slices && slice == 0; ++s) {
+                o += shared[threadIdx.x + s * colWaves * WAVE];
+            }
+            __syncthreads();
+        }
+        if (slice == 0 && n0 + lane / LANES < liveCols) {
+            const float inv = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l);
+            const int cc = ct * HT + n;
+            uint16_t *dst = a.out + ((static_cast<int64_t>(seq) * a.tokens + cc / a.group) * a.H + g * a.group + cc % a.group) * D + 4 * q;
+            u32x2 w;
+            w[0] = static_cast<uint32_t>(Narrow<BF16>(o[0] * inv)) | (static_cast<uint32_t>(Narrow<BF16>(o[1] * inv)) << 16);
+            w[1] = static_cast<uint32_t>(Narrow<BF16>(o[2] * inv)) | (static_cast<uint32_t>(Narrow<BF16>(o[3] * inv)) << 16);
+            *reinterpret_cast<u32x2 *>(dst) = w;
+        }
     }
 }
 
@@ -639,6 +838,8 @@ extern "C" int atbmi_pa_int4_decode(const AtbmiPaInt4Call *call, void *workspace
     a.maskHeadStride = call->maskHeadStride;
     a.maskRowStride = call->maskRowStride;
     a.maskLen = call->maskLen;
+    a.maskVec = ((reinterpret_cast<uintptr_t>(call->mask) & 15) == 0 &&
+                 ((call->maskSeqStride | call->maskHeadStride | call->maskRowStride) & 7) == 0) ? 1 : 0;
     a.H = call->numHeads;
     a.G = call->numKvHeads;
     a.group = call->numHeads / call->numKvHeads;
@@ -659,13 +860,23 @@ extern "C" int atbmi_pa_int4_decode(const AtbmiPaInt4Call *call, void *workspace
             constexpr int D = decltype(d)::value;
             constexpr bool BF16 = decltype(bf16)::value;
             int4kv::WithFlag(call->mask != nullptr, [&](auto mask) {
-                int4kv::PaInt4Kernel<D, BF16, decltype(mask)::value>
-                    <<<static_cast<unsigned>(grid), int4kv::PA_THREADS, 0, s>>>(a);
+                auto kernel = int4kv::PaInt4Kernel<D, BF16, decltype(mask)::value>;
+                constexpr int LDS = int4kv::PA_WAVES * (int4kv::TileLayout<D>::SLOTS * int4kv::TileLayout<D>::BYTES +
+                                                        (decltype(mask)::value ? 2048 : 0));
+                rc = ConfigureKernelLds(reinterpret_cast<const void *>(kernel), LDS);
+                if (rc == OK) {
+                    kernel<<<static_cast<unsigned>(grid), int4kv::PA_THREADS, LDS, s>>>(a);
+                }
             });
+            if (rc != OK) {
+                return;
+            }
             if (hipError_t e = hipGetLastError(); e != hipSuccess) {
                 rc = Fail(ERR_RT_FAIL, "pa_int4: launch failed: %s", hipGetErrorString(e));
             } else if (shape.merge) {
-                int4kv::PaInt4MergeKernel<D, BF16><<<static_cast<unsigned>(mergeGrid), int4kv::PA_THREADS, 0, s>>>(a);
+                // (many ranges a sequence: many parts to join for each)
+                const int threads = shape.ranges > 4 * static_cast<int64_t>(call->batch) ? int4kv::MERGE_MOST_THREADS : 256;
+                int4kv::PaInt4MergeKernel<D, BF16><<<static_cast<unsigned>(mergeGrid), threads, 0, s>>>(a);
             }
         });
     });
