@@ -20,19 +20,24 @@
 //            permuted the same way. Row m of block st is token 16 (m / 4) + 4 st + m % 4 of the 64-token tile, which
 //            leaves lane (c, kg) with the scores of tokens 16 kg .. 16 kg + 15 of column c.
 //   values   O^T = V^T P^T: A = value codes, which lie token after token (16 tokens of a channel pair are 16 bytes: a
-//            lane's tokens 16 kg .. + 15), B = the lane's own 16 weights. Nothing passes through LDS.
+//            lane's tokens 16 kg .. + 15), B = the lane's own 16 weights. With 16 columns the weights stay in the lane
+//            that has the scores; with fewer, scores and weights pass through LDS once so that no lane computes the
+//            softmax of a repeated column (batch of 64, 4 columns, 1024 to 4096 tokens: 54.4 -> 50.2 us).
 // Running maximum and sums are fp32. The maximum a column is scaled by moves only when a score exceeds it by more
 // than 2^8 (in the exponent: 8): weights up to 256 are as exact as weights up to 1, and the accumulators are rescaled
 // a few times a context instead of every tile.
 //
-// Work: the 64-token tiles of all sequences, back to back, are cut into equal ranges (an empty sequence counts as one
-// tile); a workgroup of four waves takes one range of one KV head and 16 columns, its waves every fourth tile, and
+// Work: the 64-token tiles of all sequences, back to back, each sequence behind START units that stand for what it costs
+// beyond its tiles, are cut into equal ranges (an empty sequence has one tile); a workgroup of four waves takes one range of one KV head and 16 columns, its waves every fourth tile, and
 // joins the waves' sums in LDS at the end of each sequence. A sequence inside one range is written at once; of one that
 // was cut, the parts go to fp32 partial rows (range r: part 2 r + 1 if the sequence begins in the range, else 2 r) and
 // PaInt4MergeKernel joins them. Lengths are read on the device: every workgroup adds them up for itself.
 #include <algorithm>
 #include "pa_internal.h"
 #include "int4_common.h"
+
+// (the lambdas of the kernel hold its registers: called, they would move them to memory)
+#define ATBMI_INLINE __attribute__((always_inline))
 
 namespace atbmi {
 namespace int4kv {
@@ -49,6 +54,7 @@ constexpr int PA_WAVES = 4;
 constexpr int PA_THREADS = PA_WAVES * WAVE;
 constexpr int MERGE_MOST_THREADS = 1024;
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr int START = 4;        // see UnitsOf
 constexpr float STEP_UP = 8.0f; // how far (log2) a score may exceed the reference before that moves
 
 struct PaInt4Args {
@@ -77,6 +83,8 @@ struct PaInt4Args {
     int32_t batch;
     int32_t maxBlocksPerSeq;
     int32_t blockSize;
+    int32_t tilesPerBlock;  // blockSize / 64, 0 where that is no whole number
+    uint32_t tilesMagic;    // as groupsMagic, for tilesPerBlock
     int32_t groupsPerBlock; // blockSize / 16
     uint32_t groupsMagic;   // ceil(2^32 / groupsPerBlock): x / groupsPerBlock for x * groupsPerBlock < 2^32 (0 for 1)
     int32_t numBlocks;
@@ -87,6 +95,15 @@ struct PaInt4Args {
 __device__ __forceinline__ int ContextLen(const PaInt4Args &a, int b)
 {
     return min(max(a.lens[b], 0), a.maxBlocksPerSeq * a.blockSize);
+}
+// The same through the scalar cache, for a sequence that all lanes agree on: not counted with the tiles on their way.
+template <typename T> __device__ __forceinline__ const __attribute__((address_space(4))) T *Scalar(const T *p)
+{
+    return reinterpret_cast<const __attribute__((address_space(4))) T *>(reinterpret_cast<uintptr_t>(p));
+}
+__device__ __forceinline__ int UniformLen(const PaInt4Args &a, int b)
+{
+    return min(max(Scalar(a.lens)[b], 0), a.maxBlocksPerSeq * a.blockSize);
 }
 __device__ __forceinline__ int TilesOf(int len)
 {
@@ -102,14 +119,21 @@ __device__ __forceinline__ int WaveSum(int v)
     return __builtin_amdgcn_readfirstlane(v);
 }
 
-// Ranges that get work: none shorter than a tile for each wave.
-__device__ __forceinline__ int LiveRanges(int ranges, int tiles)
+// What is cut into ranges: the tiles of a sequence behind START units that stand for none. They are what a sequence costs
+// a workgroup beyond its tiles (its first tiles are waited for, its sums are joined), so that equal ranges take equally
+// long.
+__device__ __forceinline__ int UnitsOf(int len)
 {
-    return min(ranges, (tiles + PA_WAVES - 1) / PA_WAVES);
+    return TilesOf(len) + START;
 }
-__device__ __forceinline__ int RangeBegin(int r, int tiles, int live)
+// Ranges that get work: none shorter than a tile for each wave.
+__device__ __forceinline__ int LiveRanges(int ranges, int units)
 {
-    return static_cast<int>(static_cast<int64_t>(tiles) * r / live);
+    return min(ranges, (units + PA_WAVES - 1) / PA_WAVES);
+}
+__device__ __forceinline__ int RangeBegin(int r, int units, int live)
+{
+    return static_cast<int>(static_cast<int64_t>(units) * r / live);
 }
 
 __device__ __forceinline__ float QuadMax(float x)
@@ -158,7 +182,8 @@ __device__ __forceinline__ uint32_t PackBf16(float a, float b)
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
 }
 
-// 16 bytes (4 bytes) a lane from its address to LDS at ldsAt + 16 (4) x lane, read once: not to displace anything.
+// 16 bytes (4 bytes) a lane to LDS at ldsAt + 16 (4) x lane, from an address of its own or from an offset to the wave's;
+// read once, so not to displace anything.
 __device__ __forceinline__ void ToLds16(const void *from, uint32_t ldsAt)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(ldsAt), "v"(from) : "memory", "m0");
@@ -166,6 +191,21 @@ __device__ __forceinline__ void ToLds16(const void *from, uint32_t ldsAt)
 __device__ __forceinline__ void ToLds4(const void *from, uint32_t ldsAt)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off nt" ::"s"(ldsAt), "v"(from) : "memory", "m0");
+}
+__device__ __forceinline__ void ToLds16(const void *base, uint32_t offset, uint32_t ldsAt)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(ldsAt), "v"(offset), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void ToLds4(const void *base, uint32_t offset, uint32_t ldsAt)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2 nt" ::"s"(ldsAt), "v"(offset), "s"(base) : "memory", "m0");
+}
+// Orders a wave's LDS writes before its own later reads and the other way round: a wave's LDS instructions execute in
+// order, only the compiler has to keep them.
+__device__ __forceinline__ void WaveSync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
 // A wave's tile in LDS: key codes token after token (rows of D / 2 bytes), value codes in blocks of 16 channel pairs by 64
@@ -175,30 +215,41 @@ template <int D> struct TileLayout {
     static constexpr int KEYS = TW * D / 2, VALUES = TW * D / 2;
     static constexpr int PARAMS = KEYS + VALUES;
     static constexpr int BYTES = PARAMS + 2 * TW * 4;
-    static constexpr int PIECES = D / 32; // 16-byte pieces of a key row
-    static constexpr int MOVES = 2 * (KEYS / 1024) + 2;
-    static constexpr int SLOTS = D == 64 ? 3 : 2; // tiles of a wave that are in LDS or on their way
+    static constexpr int PIECES = D / 32;           // 16-byte pieces of a key row
+    static constexpr int KEY_MOVES = KEYS / 1024;
+    static constexpr int KEY_ROWS = 1024 / (D / 2); // tokens an instruction moves
+    static constexpr int MOVES = KEY_MOVES + VALUES / 1024 + 2;
+    static constexpr int SLOTS = 2;                 // tiles of a wave that are in LDS or on their way
     // what the place of a piece is its index xor-ed with, for token `row` of 16-token group `grp`: the lanes of a read hold
     // four neighbouring rows of four groups
     static __device__ __forceinline__ int KeyTwist(int row, int grp)
     {
         return D == 64 ? (grp & 1) : (D == 128 ? ((row / 2 + grp) & 3) : ((row & 3) | ((grp & 1) << 2)));
     }
-    static constexpr int JOIN = 16 * (D + 4) * 4; // a wave's sums at the end of a sequence
-    static_assert(JOIN <= SLOTS * BYTES, "the sums take the place of the tiles");
+    static constexpr int RING = PA_WAVES * SLOTS * BYTES;
+    static constexpr int PITCH = D + 4;
+    static constexpr int JOIN_COLS = 4; // columns whose sums the waves join at a time
+    static constexpr int JOIN = PA_WAVES * JOIN_COLS * PITCH * 4;
+    static constexpr int MASKS = PA_WAVES * 2048; // a tile's mask values for each wave, in the place of the joined sums
+    static constexpr int LDS = RING + (JOIN > MASKS ? JOIN : MASKS);
 };
 
-template <int D, bool BF16, bool MASK>
+// NC: columns that the softmax is computed for, 4, 8 or 16. The matrix instruction gives 16 columns' scores, 16 of a column
+// to a lane; with fewer columns most lanes would work on repetitions. The live scores then pass through LDS (the place of
+// the tile's keys, which have been read) so that every lane has NC scores of one live column, and the weights come back
+// the same way in the matrix instruction's layout.
+template <int D, bool BF16, bool MASK, int NC>
 __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(const PaInt4Args a)
 {
     using L = TileLayout<D>;
     constexpr int KW = D / 32; // 32-bit words of a token's codes a lane holds = matrix instructions a 16-token block
     constexpr int CT = D / 32; // tiles of 16 channel pairs
-    constexpr int PITCH = D + 4;
+    constexpr int PER = WAVE / NC; // lanes that hold a column's scores
+    constexpr int WP = D == 64 ? 128 : 144; // bytes between the columns of the weights that pass through LDS
     // what the operands stand for beyond u - 7.5, and the factor of u
     constexpr float K_OFFSET = BF16 ? 23.5f : 7.5f;
     constexpr float K_FACTOR = BF16 ? 1.0f : 16777216.0f;
-    extern __shared__ __attribute__((aligned(16))) unsigned char lds[]; // a ring of tiles for each wave
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[]; // a ring of tiles for each wave, then sums or masks
     __shared__ float ldsM[PA_WAVES][HT];
     __shared__ float ldsL[PA_WAVES][HT];
 
@@ -213,31 +264,31 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
     const int ct = pair % a.colTiles;
 
     // ---- where the range begins
-    int tiles = 0;
+    int units = 0;
     for (int b = lane; b < a.batch; b += WAVE) {
-        tiles += TilesOf(ContextLen(a, b));
+        units += UnitsOf(ContextLen(a, b));
     }
-    tiles = WaveSum(tiles);
-    const int live = LiveRanges(a.ranges, tiles);
+    units = WaveSum(units);
+    const int live = LiveRanges(a.ranges, units);
     if (range >= live) {
         return;
     }
-    const int begin = RangeBegin(range, tiles, live);
-    const int end = RangeBegin(range + 1, tiles, live);
-    int seq = 0, before = 0; // the sequence that holds tile `begin`, tiles of the sequences before it
+    const int begin = RangeBegin(range, units, live);
+    const int end = RangeBegin(range + 1, units, live);
+    int seq = 0, before = 0; // the sequence that holds unit `begin`, units of the sequences before it
     for (int b0 = 0;; b0 += WAVE) {
-        const int mine = b0 + lane < a.batch ? TilesOf(ContextLen(a, b0 + lane)) : 0;
-        int upTo = mine;
+        const int own = b0 + lane < a.batch ? UnitsOf(ContextLen(a, b0 + lane)) : 0;
+        int upTo = own;
 #pragma unroll
         for (int step = 1; step < WAVE; step *= 2) {
             const int other = __shfl_up(upTo, step);
             upTo += lane >= step ? other : 0;
         }
         const uint64_t past = __ballot(before + upTo > begin);
-        if (past != 0) { // (begin < tiles: some sequence holds it)
+        if (past != 0) { // (begin < units: some sequence holds it)
             const int at = __builtin_ctzll(past);
             seq = b0 + at;
-            before += __shfl(upTo - mine, at);
+            before += __shfl(upTo - own, at);
             break;
         }
         before += __shfl(upTo, WAVE - 1);
@@ -246,28 +297,62 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
     before = __builtin_amdgcn_readfirstlane(before);
 
     const int columns = a.group * a.tokens;
-    const int col = min(ct * HT + c, columns - 1); // (lanes past the last column repeat it; nothing of theirs is stored)
-    const int qTok = col / a.group;
-    const int qHead = g * a.group + col % a.group;
     const int liveCols = min(HT, columns - ct * HT);
+    auto columnOf = [&](int n) { return min(ct * HT + n, columns - 1); }; // (past the last one: the last again, not stored)
+    const int col = columnOf(c);             // of the matrix instruction's lane
+    const int sl = NC == 16 ? c : lane / PER; // the column whose scores the lane works on, and the first of its NC tokens
+    const int tok0 = NC == 16 ? 16 * kg : lane % PER * NC;
+    const int sCol = columnOf(sl);
     unsigned char *mine = lds + wave * L::SLOTS * L::BYTES;
     const uint32_t mineAt = LdsAddress(mine);
-    const uint32_t maskAt = LdsAddress(lds + PA_WAVES * L::SLOTS * L::BYTES + wave * 2048); // MASK only
+    float *const sums = reinterpret_cast<float *>(lds + L::RING); // [waves][JOIN_COLS][PITCH]
+    unsigned char *const masks = lds + L::RING + wave * 2048;     // [NC][64] (MASK only)
+    const uint32_t maskAt = LdsAddress(masks);
 
-    for (int at = begin; at < end;) {
-        const int len = ContextLen(a, seq);
-        const int seqTiles = TilesOf(len);
-        const int tBegin = at - before;
-        const int tEnd = min(seqTiles, end - before);
-        // (read through the scalar cache: block ids are not counted with the tiles on their way)
-        const auto *table = reinterpret_cast<const __attribute__((address_space(4))) int32_t *>(
-            reinterpret_cast<uintptr_t>(a.tables + static_cast<int64_t>(seq) * a.maxBlocksPerSeq));
+    // where a lane reads in a tile that lies in one block: offsets from the tile's first key, value and param
+    uint32_t keyAt[L::KEY_MOVES];
+#pragma unroll
+    for (int i = 0; i < L::KEY_MOVES; ++i) {
+        const int token = L::KEY_ROWS * i + lane / L::PIECES;
+        keyAt[i] = token * (D / 2) + ((lane % L::PIECES) ^ L::KeyTwist(token % 16, token / 16)) * 16;
+    }
+    const int vGrp = (lane % 4) ^ (lane / 8 % 4);
+    const uint32_t valueAt = lane / 4 * a.blockSize + 16 * vGrp;
+    const int64_t headBytes = static_cast<int64_t>(a.blockSize) * (D / 2);
+
+    for (;;) {
+        const int len = UniformLen(a, seq);
+        const int tBegin = max(max(begin - before, 0) - START, 0);
+        const int tEnd = max(min(end - before, UnitsOf(len)) - START, tBegin);
+        // (block ids are read through the scalar cache: not counted with the tiles on their way)
+        const auto *table = Scalar(a.tables + static_cast<int64_t>(seq) * a.maxBlocksPerSeq);
 
         // ---- asks for tile t; returns which of its four 16-token groups lie in blocks that exist, as bits
-        auto request = [&](int t, int slot) {
+        auto request = [&](int t, int slot) ATBMI_INLINE -> uint32_t {
             const uint32_t to = mineAt + slot * L::BYTES;
+            if (a.tilesPerBlock > 0) { // a block holds whole tiles
+                const uint32_t at = a.tilesMagic ? static_cast<uint32_t>((static_cast<uint64_t>(t) * a.tilesMagic) >> 32) : t;
+                const int id = table[min(static_cast<int>(at), a.maxBlocksPerSeq - 1)];
+                const bool ok = id >= 0 && id < a.numBlocks;
+                const int64_t head = static_cast<int64_t>(ok ? id : 0) * a.G + g;
+                const int place = (t - static_cast<int>(at) * a.tilesPerBlock) * TW;
+                const uint8_t *k = a.kc + head * headBytes + place * (D / 2);
+                const uint8_t *v = a.vc + head * headBytes + place;
+#pragma unroll
+                for (int i = 0; i < L::KEY_MOVES; ++i) {
+                    ToLds16(k, keyAt[i], to + i * 1024);
+                }
+#pragma unroll
+                for (int i = 0; i < CT; ++i) {
+                    ToLds16(v + i * 16 * a.blockSize, valueAt, to + L::KEYS + i * 1024);
+                }
+                const int64_t param = head * a.blockSize + place;
+                ToLds4(a.kp + param, 4 * lane, to + L::PARAMS);
+                ToLds4(a.vp + param, 4 * lane, to + L::PARAMS + TW * 4);
+                return ok ? 15u : 0u;
+            }
             uint32_t there = 0;
-            int64_t first[4]; // of a group: its block's head, counted in rows of blockSize tokens
+            int64_t first[4]; // of a group: its block's head
             int place[4];     // and its first token within the block
 #pragma unroll
             for (int grp = 0; grp < 4; ++grp) {
@@ -279,26 +364,23 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
                 first[grp] = static_cast<int64_t>(ok ? id : 0) * a.G + g;
                 place[grp] = static_cast<int>(x - at16 * a.groupsPerBlock) * 16;
             }
-            auto headOf = [&](int grp) { // (a lane's own choice of four values of the wave)
+            auto headOf = [&](int grp) ATBMI_INLINE { // (a lane's own choice of four values of the wave)
                 const int64_t lo = grp == 0 ? first[0] : int64_t(first[1]), hi = grp == 2 ? first[2] : int64_t(first[3]);
                 return grp < 2 ? lo : int64_t(hi);
             };
-            auto placeOf = [&](int grp) {
+            auto placeOf = [&](int grp) ATBMI_INLINE {
                 const int lo = grp == 0 ? place[0] : int(place[1]), hi = grp == 2 ? place[2] : int(place[3]);
                 return grp < 2 ? lo : int(hi);
             };
 #pragma unroll
-            for (int i = 0; i < L::KEYS / 1024; ++i) {
-                constexpr int ROWS = 1024 / (D / 2); // tokens an instruction moves
-                const int token = ROWS * i + lane / L::PIECES;
-                const int grp = token / 16, row = token % 16;
-                const int piece = (lane % L::PIECES) ^ L::KeyTwist(row, grp);
-                const int64_t head = ROWS <= 16 ? first[ROWS * i / 16 % 4] : headOf(grp);
-                const int in = ROWS <= 16 ? place[ROWS * i / 16 % 4] : placeOf(grp);
-                ToLds16(a.kc + (head * a.blockSize + in + row) * (D / 2) + piece * 16, to + i * 1024);
+            for (int i = 0; i < L::KEY_MOVES; ++i) {
+                const int token = L::KEY_ROWS * i + lane / L::PIECES;
+                const int grp = token / 16;
+                const int64_t head = L::KEY_ROWS <= 16 ? first[L::KEY_ROWS * i / 16 % 4] : headOf(grp);
+                const int in = L::KEY_ROWS <= 16 ? place[L::KEY_ROWS * i / 16 % 4] : placeOf(grp);
+                ToLds16(a.kc + head * headBytes + in * (D / 2) + (keyAt[i] - 16 * grp * (D / 2)), to + i * 1024);
             }
-            const int vGrp = (lane % 4) ^ (lane / 8 % 4);
-            const uint8_t *v = a.vc + (headOf(vGrp) * (D / 2) + lane / 4) * a.blockSize + placeOf(vGrp);
+            const uint8_t *v = a.vc + headOf(vGrp) * headBytes + placeOf(vGrp) + (valueAt - 16 * vGrp);
 #pragma unroll
             for (int i = 0; i < CT; ++i) {
                 ToLds16(v + static_cast<int64_t>(16 * i) * a.blockSize, to + L::KEYS + i * 1024);
@@ -312,7 +394,7 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
         // ---- the query columns, permuted as Spread orders the codes, and their sums
         u32x4 q[KW];
         float sumQ = 0.0f;
-        const uint16_t *qRow = a.q + (static_cast<int64_t>(seq) * a.tokens + qTok) * a.H * D + static_cast<int64_t>(qHead) * D + kg * (D / 4);
+        const uint16_t *qRow = a.q + ((static_cast<int64_t>(seq) * a.tokens + col / a.group) * a.H + g * a.group + col % a.group) * D + kg * (D / 4);
 #pragma unroll
         for (int i = 0; i < KW; ++i) {
             const u32x4 w = *reinterpret_cast<const u32x4 *>(qRow + 8 * i);
@@ -324,12 +406,18 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
                          __builtin_amdgcn_perm(w[3], w[1], 0x05040100u), __builtin_amdgcn_perm(w[3], w[1], 0x07060302u)};
         }
         sumQ = QuadSum(sumQ);
+        if constexpr (NC < 16) {
+            sumQ = __shfl(sumQ, sl);
+        }
         const float midQ = sumQ * a.scale2;
         const float offQ = -K_OFFSET * sumQ * a.scale2;
         const float facQ = K_FACTOR * a.scale2;
-        const int seen = len - a.tokens + 1 + qTok; // positions this column sees
-        const int allSee = len - a.tokens + 1;      // positions every column sees
-        const uint16_t *maskRow = MASK ? a.mask + seq * a.maskSeqStride + qHead * a.maskHeadStride + qTok * a.maskRowStride : nullptr;
+        const int seen = len - a.tokens + 1 + sCol / a.group; // positions the lane's column sees
+        const int allSee = len - a.tokens + 1;                // positions every column sees
+        auto maskRowOf = [&](int column) ATBMI_INLINE {
+            return a.mask + seq * a.maskSeqStride + (g * a.group + column % a.group) * a.maskHeadStride +
+                   column / a.group * a.maskRowStride;
+        };
 
         f32x4 acc[CT][2]; // [..][0]: even channels of the pairs, [1]: odd ones
         f32x4 ones = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -337,70 +425,52 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
         for (int i = 0; i < CT; ++i) {
             acc[i][0] = acc[i][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        float top = -INFINITY; // the reference (log2)
+        float top = -INFINITY; // the reference (log2) of the lane's column
         float total = 0.0f;    // of the lane's own tokens
         float mids = 0.0f;
 
-        // Mask values of the lane's 16 tokens of a tile, two a word. Rows on 16-byte boundaries come through LDS, asked for a
-        // tile ahead; others, and those of the tile in which the mask ends, are read where they are used.
-        auto maskAhead = [&](int t) { return a.maskVec != 0 && (t + 1) * TW <= a.maskLen; };
-        auto requestMask = [&](int t) {
-            const uint16_t *m = maskRow + t * TW + 16 * kg;
-            ToLds16(m, maskAt);
-            ToLds16(m + 8, maskAt + 1024);
-        };
-        auto readMask = [&](int t, uint32_t (&m)[8]) {
-            if (maskAhead(t)) {
+        // Mask values. Rows on 16-byte boundaries come through LDS, asked for a tile ahead (eight lanes a column); others, and
+        // those of a sequence's first tile and of the one in which the mask ends, are read where they are used.
+        bool maskThere = false;
+        auto maskAhead = [&](int t) ATBMI_INLINE { return a.maskVec != 0 && (t + 1) * TW <= a.maskLen; };
+        auto requestMask = [&](int t) ATBMI_INLINE {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const u32x4 w = *reinterpret_cast<const u32x4 *>(lds + PA_WAVES * L::SLOTS * L::BYTES + wave * 2048 + 1024 * i + 16 * lane);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        m[4 * i + e] = w[e];
-                    }
-                }
-            } else {
-                const int first = t * TW + 16 * kg;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint32_t lo = maskRow[min(first + 2 * i, a.maskLen - 1)];
-                    const uint32_t hi = maskRow[min(first + 2 * i + 1, a.maskLen - 1)];
-                    m[i] = lo | (hi << 16);
+            for (int i = 0; i < (NC + 7) / 8; ++i) {
+                if (NC >= 8 || lane < 8 * NC) {
+                    ToLds16(maskRowOf(columnOf(lane / 8 + 8 * i)) + t * TW + lane % 8 * 8, maskAt + i * 1024);
                 }
             }
         };
 
         uint32_t there[L::SLOTS];
-        if constexpr (MASK) {
-            if (tBegin + wave < tEnd && maskAhead(tBegin + wave)) {
-                requestMask(tBegin + wave);
-            }
-        }
 #pragma unroll
         for (int i = 0; i < L::SLOTS; ++i) {
-            there[i] = 0;
             const int t = tBegin + wave + i * PA_WAVES;
-            if (t < tEnd) {
-                there[i] = request(t, i);
-            }
+            there[i] = t < tEnd ? request(t, i) : 0;
         }
 
         // (HIDDEN: some token of the tile may be hidden from some column)
-        auto tile = [&](int t, int slot, uint32_t ok4, auto hidden) {
+        auto tile = [&](int t, int slot, auto hidden) ATBMI_INLINE {
             constexpr bool HIDDEN = MASK || decltype(hidden)::value;
-            const int t0 = t * TW;
-            const unsigned char *from = mine + slot * L::BYTES;
-            const int first = t0 + 16 * kg;
-            uint32_t maskBits[8];
+            unsigned char *from = mine + slot * L::BYTES;
+            const int first = t * TW + tok0;
+            float bias[MASK ? NC : 1];
             if constexpr (MASK) {
-                readMask(t, maskBits);
+                const uint16_t *row = maskRowOf(sCol);
+#pragma unroll
+                for (int j = 0; j < NC; ++j) {
+                    const uint16_t m = maskThere ? *reinterpret_cast<const uint16_t *>(masks + sl * 128 + (tok0 + j) * 2)
+                                                 : row[min(first + j, a.maskLen - 1)];
+                    bias[j] = first + j < a.maskLen ? Widen<BF16>(m) : -INFINITY;
+                }
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                if (t + PA_WAVES < tEnd && maskAhead(t + PA_WAVES)) {
+                maskThere = t + PA_WAVES < tEnd && maskAhead(t + PA_WAVES);
+                if (maskThere) {
                     requestMask(t + PA_WAVES);
                 }
             }
-            // ---- scores of tokens t0 + 16 kg + j, in log2 units
-            float s[16];
+            // ---- q . u of 16 tokens a column to a lane: tokens 16 kg + 4 st + e
+            f32x4 dot[4];
 #pragma unroll
             for (int st = 0; st < 4; ++st) {
                 const int row = 4 * st + (c & 3), grp = c >> 2;
@@ -415,47 +485,83 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
                         __builtin_memcpy(kw + 4 * i, __builtin_assume_aligned(kr + ((D / 128 * kg + i) ^ twist) * 16, 16), 16);
                     }
                 }
-                f32x4 dot = {0.0f, 0.0f, 0.0f, 0.0f};
+                dot[st] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int i = 0; i < KW; ++i) {
-                    dot = Mfma<BF16>(Spread<BF16>(kw[i]), q[i], dot);
+                    dot[st] = Mfma<BF16>(Spread<BF16>(kw[i]), q[i], dot[st]);
                 }
-                const u32x4 kpw = *reinterpret_cast<const u32x4 *>(from + L::PARAMS + 64 * kg + 16 * st);
+            }
+            // ---- the lane's scores, in log2 units
+            float s[NC];
+            if constexpr (NC == 16) {
+#pragma unroll
+                for (int j = 0; j < NC; ++j) {
+                    s[j] = dot[j / 4][j % 4];
+                }
+            } else {
+                WaveSync();
+                if (c < NC) {
+#pragma unroll
+                    for (int st = 0; st < 4; ++st) {
+                        *reinterpret_cast<f32x4 *>(from + c * 256 + 64 * kg + 16 * st) = dot[st];
+                    }
+                }
+                WaveSync();
+#pragma unroll
+                for (int j = 0; j < NC; j += 4) {
+                    const f32x4 x = *reinterpret_cast<const f32x4 *>(from + sl * 256 + (tok0 + j) * 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[j + e] = x[e];
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < NC; j += 4) {
+                const u32x4 word = *reinterpret_cast<const u32x4 *>(from + L::PARAMS + (tok0 + j) * 4);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    s[4 * st + e] = __builtin_fmaf(ScaleOf<BF16>(kpw[e]), __builtin_fmaf(dot[e], facQ, offQ), MidOf<BF16>(kpw[e]) * midQ);
+                    s[j + e] = __builtin_fmaf(ScaleOf<BF16>(word[e]), __builtin_fmaf(s[j + e], facQ, offQ), MidOf<BF16>(word[e]) * midQ);
                 }
             }
             if constexpr (MASK) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const float m = Widen<BF16>(static_cast<uint16_t>(maskBits[j / 2] >> (16 * (j % 2))));
+                for (int j = 0; j < NC; ++j) {
                     // (the lowest finite value leaves fp32 when it is turned into log2 units: it stays finite here, so that
                     // a row of nothing else is the mean of its values; NaN stays NaN)
-                    float v = __builtin_fmaf(m, LOG2E, s[j]);
+                    float v = __builtin_fmaf(bias[j], LOG2E, s[j]);
                     v = v < -3.0e38f ? -3.0e38f : v;
-                    s[j] = (m == -INFINITY || first + j >= a.maskLen) ? -INFINITY : v;
+                    s[j] = bias[j] == -INFINITY ? -INFINITY : v;
                 }
             }
             if constexpr (HIDDEN) {
-                const bool ok = ((ok4 >> kg) & 1) != 0;
+                const uint32_t ok4 = there[slot];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
+                for (int j = 0; j < NC; ++j) {
+                    const bool ok = ((ok4 >> (NC == 16 ? kg : (tok0 + j) / 16)) & 1) != 0;
                     s[j] = ok && first + j < seen ? s[j] : -INFINITY;
                 }
             }
             // ---- weights
             float most = s[0];
 #pragma unroll
-            for (int j = 1; j < 16; ++j) {
+            for (int j = 1; j < NC; ++j) {
                 most = fmaxf(most, s[j]);
             }
             if (__ballot(most > top + STEP_UP || (top == -INFINITY && most > -INFINITY)) != 0) {
-                const float newTop = fmaxf(top, QuadMax(most));
-                const float keep = top == -INFINITY ? 0.0f : exp2f(top - newTop);
+                float newTop = most;
+#pragma unroll
+                for (int step = NC == 16 ? 16 : 1; step < (NC == 16 ? WAVE : PER); step *= 2) {
+                    newTop = fmaxf(newTop, __shfl_xor(newTop, step));
+                }
+                newTop = fmaxf(top, newTop);
+                float keep = top == -INFINITY ? 0.0f : exp2f(top - newTop);
                 top = newTop;
                 total *= keep;
                 mids *= keep;
+                if constexpr (NC < 16) {
+                    keep = __shfl(keep, c % NC * PER);
+                }
                 ones *= keep;
 #pragma unroll
                 for (int i = 0; i < CT; ++i) {
@@ -464,13 +570,13 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
                 }
             }
             const float base = top == -INFINITY ? 0.0f : top;
-            float pv[16];
+            float pv[NC];
 #pragma unroll
-            for (int j4 = 0; j4 < 4; ++j4) {
-                const u32x4 vpw = *reinterpret_cast<const u32x4 *>(from + L::PARAMS + TW * 4 + 64 * kg + 16 * j4);
+            for (int j4 = 0; j4 < NC; j4 += 4) {
+                const u32x4 vpw = *reinterpret_cast<const u32x4 *>(from + L::PARAMS + TW * 4 + (tok0 + j4) * 4);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int j = 4 * j4 + e;
+                    const int j = j4 + e;
                     const float p = __builtin_amdgcn_exp2f(s[j] - base);
                     total += p;
                     // (a hidden token's params may hold anything: 0 times them must be 0)
@@ -481,18 +587,47 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
             }
             // ---- values. The weights (times the value scale) are rounded to bf16, which has fp32's range whatever the
             // scales are: an error of at most 2^-8 each for bf16 models, whose output is rounded as coarsely; for fp16
-            // models the remainder is multiplied as well (2^-16 left).
-            u32x4 pw[2], pr[2];
+            // models the remainder is multiplied as well (2^-16 left). Tokens j and j + 2 share a register, as Spread
+            // leaves them.
+            u32x4 pw[2], pr[2]; // tokens 16 kg + 8 h .. + 7
+            uint32_t packed[NC / 2], rest[NC / 2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int e = 0; e < NC / 2; ++e) {
+                const int j = 4 * (e / 2) + e % 2;
+                packed[e] = PackBf16(pv[j], pv[j + 2]);
+                if constexpr (!BF16) {
+                    rest[e] = PackBf16(pv[j] - __uint_as_float(packed[e] << 16), pv[j + 2] - __uint_as_float(packed[e] & 0xffff0000u));
+                }
+            }
+            if constexpr (NC == 16) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int j = 8 * h + 4 * (e / 2) + e % 2; // tokens j and j + 2 share a register, as Spread leaves them
-                    pw[h][e] = PackBf16(pv[j], pv[j + 2]);
+                for (int e = 0; e < 8; ++e) {
+                    pw[e / 4][e % 4] = packed[e];
                     if constexpr (!BF16) {
-                        pr[h][e] = PackBf16(pv[j] - __uint_as_float(pw[h][e] << 16), pv[j + 2] - __uint_as_float(pw[h][e] & 0xffff0000u));
+                        pr[e / 4][e % 4] = rest[e];
                     }
                 }
+            } else {
+                // (rows of WP bytes a column, 16 more than they hold where there is room; the scores have been read)
+                WaveSync();
+#pragma unroll
+                for (int e = 0; e < NC / 2; e += 2) {
+                    *reinterpret_cast<u32x2 *>(from + sl * WP + tok0 * 2 + e * 4) = u32x2{packed[e], packed[e + 1]};
+                    if constexpr (!BF16) {
+                        *reinterpret_cast<u32x2 *>(from + (NC + sl) * WP + tok0 * 2 + e * 4) = u32x2{rest[e], rest[e + 1]};
+                    }
+                }
+                WaveSync();
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    pw[h] = *reinterpret_cast<const u32x4 *>(from + c % NC * WP + 32 * kg + 16 * h);
+                    if constexpr (!BF16) {
+                        pr[h] = *reinterpret_cast<const u32x4 *>(from + (NC + c % NC) * WP + 32 * kg + 16 * h);
+                    }
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
                 constexpr uint32_t ONE = 0x3f803f80u;
                 const u32x4 one = {ONE, ONE, ONE, ONE};
                 ones = Mfma<true>(one, pw[h], ones);
@@ -518,23 +653,22 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
             }
         };
 
-        // ---- tiles. A slot is waited for by the number of loads that were asked for behind it (with a mask: behind the
-        // tile's mask values, which are asked for after all tiles but the last).
-        constexpr int BEHIND = MASK ? L::MOVES : (L::SLOTS - 1) * L::MOVES;
+        // ---- tiles. A slot is waited for by the number of loads that were asked for behind it (mask values are asked for
+        // in front of the tile that is the last behind).
         for (int t = tBegin + wave; t < tEnd; t += L::SLOTS * PA_WAVES) {
 #pragma unroll
             for (int i = 0; i < L::SLOTS; ++i) {
                 const int now = t + i * PA_WAVES;
                 if (now < tEnd) {
                     if (now + (L::SLOTS - 1) * PA_WAVES < tEnd) {
-                        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(BEHIND) : "memory");
+                        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((L::SLOTS - 1) * L::MOVES) : "memory");
                     } else {
                         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                     }
                     if (!MASK && (now + 1) * TW <= allSee && there[i] == 15u) {
-                        tile(now, i, 15u, std::false_type{});
+                        tile(now, i, std::false_type{});
                     } else {
-                        tile(now, i, there[i], std::true_type{});
+                        tile(now, i, std::true_type{});
                     }
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the slot has been read
                     const int later = now + L::SLOTS * PA_WAVES;
@@ -545,76 +679,93 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
             }
         }
 
-        // ---- join the waves
-        total = QuadSum(total);
-        mids = QuadSum(mids);
-        const int busy = min(PA_WAVES, tEnd - tBegin);
-        auto sums = [&](int w) { return reinterpret_cast<float *>(lds + w * L::SLOTS * L::BYTES); }; // [16][PITCH]
-        if (kg == 0) {
-            ldsM[wave][c] = top;
-        }
-        __syncthreads();
-        float joint = -INFINITY;
-        for (int w = 0; w < busy; ++w) {
-            joint = fmaxf(joint, ldsM[w][c]);
-        }
-        const float f = top == -INFINITY ? 0.0f : exp2f(top - joint);
-        if (wave < busy) {
+        // ---- join the waves, four columns at a time
+        if (tEnd > tBegin) {
+            if constexpr (NC == 16) {
+                total = QuadSum(total);
+                mids = QuadSum(mids);
+            } else {
+#pragma unroll
+                for (int step = 1; step < PER; step *= 2) {
+                    total += __shfl_xor(total, step);
+                    mids += __shfl_xor(mids, step);
+                }
+                total = __shfl(total, c % NC * PER);
+                mids = __shfl(mids, c % NC * PER);
+                top = __shfl(top, c % NC * PER);
+            }
+            __syncthreads(); // (mask values in the place of the sums, and the maxima of the sequence before, have been read)
+            if (kg == 0) {
+                ldsM[wave][c] = top;
+            }
+            __syncthreads();
+            float joint = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < PA_WAVES; ++w) {
+                joint = fmaxf(joint, ldsM[w][c]);
+            }
+            const bool none = top == -INFINITY;
+            const float f = none ? 0.0f : exp2f(top - joint);
             if (kg == 0) {
                 ldsL[wave][c] = total * f;
             }
             const float rest = mids - 23.5f * ones[0];
+            const bool whole = tBegin == 0 && tEnd == TilesOf(len);
+            const int64_t part = static_cast<int64_t>(2 * range + (tBegin == 0 ? 1 : 0)) * pairs + pair;
+            for (int n0 = 0; n0 < liveCols; n0 += L::JOIN_COLS) {
+                if (c / L::JOIN_COLS == n0 / L::JOIN_COLS) {
+                    float *to = sums + (wave * L::JOIN_COLS + c % L::JOIN_COLS) * L::PITCH + 8 * kg;
 #pragma unroll
-            for (int i = 0; i < CT; ++i) {
-                float *to = sums(wave) + c * PITCH + 32 * i + 8 * kg;
+                    for (int i = 0; i < CT; ++i) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    to[2 * e] = top == -INFINITY ? 0.0f : (acc[i][0][e] + rest) * f;
-                    to[2 * e + 1] = top == -INFINITY ? 0.0f : (acc[i][1][e] + rest) * f;
+                        for (int e = 0; e < 4; ++e) {
+                            to[32 * i + 2 * e] = none ? 0.0f : (acc[i][0][e] + rest) * f;
+                            to[32 * i + 2 * e + 1] = none ? 0.0f : (acc[i][1][e] + rest) * f;
+                        }
+                    }
                 }
-            }
-        }
-        __syncthreads();
-        const bool whole = tBegin == 0 && tEnd == seqTiles;
-        const int64_t part = static_cast<int64_t>(2 * range + (tBegin == 0 ? 1 : 0)) * pairs + pair;
-        for (int i = threadIdx.x; i < liveCols * (D / 4); i += PA_THREADS) {
-            const int n = i / (D / 4);
-            const int d = i % (D / 4) * 4;
-            f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-            float l = 0.0f;
-            for (int w = 0; w < busy; ++w) {
-                o += *reinterpret_cast<const f32x4 *>(sums(w) + n * PITCH + d);
-                l += ldsL[w][n];
-            }
-            if (whole) {
-                const float inv = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l); // nothing seen: zeros; NaN stays
-                const int cc = ct * HT + n;
-                uint16_t *dst = a.out + ((static_cast<int64_t>(seq) * a.tokens + cc / a.group) * a.H + g * a.group + cc % a.group) * D + d;
-                u32x2 w;
-                w[0] = static_cast<uint32_t>(Narrow<BF16>(o[0] * inv)) | (static_cast<uint32_t>(Narrow<BF16>(o[1] * inv)) << 16);
-                w[1] = static_cast<uint32_t>(Narrow<BF16>(o[2] * inv)) | (static_cast<uint32_t>(Narrow<BF16>(o[3] * inv)) << 16);
-                *reinterpret_cast<u32x2 *>(dst) = w;
-            } else {
-                *reinterpret_cast<f32x4 *>(a.partO + (part * HT + n) * D + d) = o;
-                if (d == 0) {
-                    a.partL[part * HT + n] = l;
+                __syncthreads();
+                const int n = n0 + static_cast<int>(threadIdx.x) / (D / 4);
+                if (static_cast<int>(threadIdx.x) < L::JOIN_COLS * (D / 4) && n < liveCols) {
+                    const int d = static_cast<int>(threadIdx.x) % (D / 4) * 4;
+                    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+                    float l = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < PA_WAVES; ++w) {
+                        o += *reinterpret_cast<const f32x4 *>(sums + (w * L::JOIN_COLS + n - n0) * L::PITCH + d);
+                        l += ldsL[w][n];
+                    }
+                    if (whole) {
+                        const float inv = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l); // nothing seen: zeros; NaN stays
+                        const int cc = ct * HT + n;
+                        uint16_t *dst = a.out + ((static_cast<int64_t>(seq) * a.tokens + cc / a.group) * a.H + g * a.group + cc % a.group) * D + d;
+                        u32x2 w;
+                        w[0] = static_cast<uint32_t>(Narrow<BF16>(o[0] * inv)) | (static_cast<uint32_t>(Narrow<BF16>(o[1] * inv)) << 16);
+                        w[1] = static_cast<uint32_t>(Narrow<BF16>(o[2] * inv)) | (static_cast<uint32_t>(Narrow<BF16>(o[3] * inv)) << 16);
+                        *reinterpret_cast<u32x2 *>(dst) = w;
+                    } else {
+                        *reinterpret_cast<f32x4 *>(a.partO + (part * HT + n) * D + d) = o;
+                        if (d == 0) {
+                            float m = -INFINITY;
+#pragma unroll
+                            for (int w = 0; w < PA_WAVES; ++w) {
+                                m = fmaxf(m, ldsM[w][n]);
+                            }
+                            a.partL[part * HT + n] = l;
+                            a.partM[part * HT + n] = m;
+                        }
+                    }
                 }
+                __syncthreads();
             }
-        }
-        if (!whole && threadIdx.x < liveCols) {
-            float m = -INFINITY;
-            for (int w = 0; w < busy; ++w) {
-                m = fmaxf(m, ldsM[w][threadIdx.x]);
-            }
-            a.partM[part * HT + threadIdx.x] = m;
-        }
-        before += seqTiles;
-        at = before;
-        ++seq;
-        if (at < end) {
+            // (stores are counted with loads: the next sequence's tiles are waited for by the number behind them)
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads(); // (the sums have been read: tiles may take their place)
         }
+        before += UnitsOf(len);
+        if (before >= end) {
+            return;
+        }
+        ++seq;
     }
 }
 
@@ -634,21 +785,20 @@ template <int D, bool BF16> __global__ __launch_bounds__(MERGE_MOST_THREADS) voi
     const int pair = blockIdx.x % pairs;
     const int g = pair / a.colTiles;
     const int ct = pair % a.colTiles;
-    int tiles = 0, before = 0;
+    int units = 0, before = 0;
     for (int b = lane; b < a.batch; b += WAVE) {
-        const int mine = TilesOf(ContextLen(a, b));
-        tiles += mine;
-        before += b < seq ? mine : 0;
+        const int own = UnitsOf(ContextLen(a, b));
+        units += own;
+        before += b < seq ? own : 0;
     }
-    tiles = WaveSum(tiles);
+    units = WaveSum(units);
     before = WaveSum(before);
-    const int live = LiveRanges(a.ranges, tiles);
-    const int last = before + TilesOf(ContextLen(a, seq)) - 1;
-    auto rangeOf = [&](int tile) { // the range r with begin(r) <= tile < begin(r + 1)
-        return static_cast<int>(((static_cast<int64_t>(tile) + 1) * live - 1) / tiles);
+    const int live = LiveRanges(a.ranges, units);
+    auto rangeOf = [&](int unit) { // the range r with begin(r) <= unit < begin(r + 1)
+        return static_cast<int>(((static_cast<int64_t>(unit) + 1) * live - 1) / units);
     };
-    const int r0 = rangeOf(before);
-    const int parts = rangeOf(last) - r0 + 1;
+    const int r0 = rangeOf(before + START); // (of the sequence's first tile)
+    const int parts = rangeOf(before + UnitsOf(ContextLen(a, seq)) - 1) - r0 + 1;
     if (parts == 1) {
         return;
     }
@@ -727,7 +877,7 @@ int CheckCall(const AtbmiPaInt4Call *c)
     }
     // (tiles of all sequences are counted in 32 bits)
     const int64_t mostTiles = (static_cast<int64_t>(c->maxBlocksPerSeq) * c->blockSize + TW - 1) / TW;
-    if (mostTiles * c->batch > 0x7fffffffLL) {
+    if ((mostTiles + START) * c->batch > 0x7fffffffLL) {
         return Fail(ERR_INVALID_PARAM, "pa_int4: %d sequences of up to %lld tokens are more than one call takes", c->batch,
                     (long long)mostTiles * TW);
     }
@@ -758,7 +908,7 @@ PaInt4Shape ShapeOf(const AtbmiPaInt4Call *c)
     const int64_t mostTiles = (static_cast<int64_t>(c->maxBlocksPerSeq) * c->blockSize + TW - 1) / TW;
     const int64_t perCu = c->headDim == 256 ? 1 : 2; // workgroups a CU holds at once (registers)
     s.ranges = std::max<int64_t>(1, DeviceComputeUnits() * perCu / s.pairs);
-    s.ranges = std::min<int64_t>(s.ranges, std::max<int64_t>(1, (mostTiles * c->batch + PA_WAVES - 1) / PA_WAVES));
+    s.ranges = std::min<int64_t>(s.ranges, std::max<int64_t>(1, ((mostTiles + START) * c->batch + PA_WAVES - 1) / PA_WAVES));
     s.merge = s.ranges > 1 && mostTiles > 1;
     if (s.merge) {
         const uint64_t rows = static_cast<uint64_t>(2 * s.ranges * s.pairs) * HT;
@@ -848,8 +998,11 @@ extern "C" int atbmi_pa_int4_decode(const AtbmiPaInt4Call *call, void *workspace
     a.batch = call->batch;
     a.maxBlocksPerSeq = call->maxBlocksPerSeq;
     a.blockSize = call->blockSize;
+    auto magic = [](int32_t d) { return d <= 1 ? 0 : static_cast<uint32_t>(((1ULL << 32) + d - 1) / d); };
+    a.tilesPerBlock = call->blockSize % int4kv::TW == 0 ? call->blockSize / int4kv::TW : 0;
+    a.tilesMagic = magic(a.tilesPerBlock);
     a.groupsPerBlock = call->blockSize / 16;
-    a.groupsMagic = a.groupsPerBlock == 1 ? 0 : static_cast<uint32_t>(((1ULL << 32) + a.groupsPerBlock - 1) / a.groupsPerBlock);
+    a.groupsMagic = magic(a.groupsPerBlock);
     a.numBlocks = call->numBlocks;
     a.ranges = static_cast<int32_t>(shape.ranges);
     a.scale2 = call->qkScale * int4kv::LOG2E;
@@ -859,13 +1012,22 @@ extern "C" int atbmi_pa_int4_decode(const AtbmiPaInt4Call *call, void *workspace
         int4kv::WithFlag(call->dtype == ATBMI_BF16, [&](auto bf16) {
             constexpr int D = decltype(d)::value;
             constexpr bool BF16 = decltype(bf16)::value;
-            int4kv::WithFlag(call->mask != nullptr, [&](auto mask) {
-                auto kernel = int4kv::PaInt4Kernel<D, BF16, decltype(mask)::value>;
-                constexpr int LDS = int4kv::PA_WAVES * (int4kv::TileLayout<D>::SLOTS * int4kv::TileLayout<D>::BYTES +
-                                                        (decltype(mask)::value ? 2048 : 0));
+            auto launch = [&](auto mask, auto nc) {
+                auto kernel = int4kv::PaInt4Kernel<D, BF16, decltype(mask)::value, decltype(nc)::value>;
+                constexpr int LDS = int4kv::TileLayout<D>::LDS;
                 rc = ConfigureKernelLds(reinterpret_cast<const void *>(kernel), LDS);
                 if (rc == OK) {
                     kernel<<<static_cast<unsigned>(grid), int4kv::PA_THREADS, LDS, s>>>(a);
+                }
+            };
+            int4kv::WithFlag(call->mask != nullptr, [&](auto mask) {
+                const int columns = a.group * a.tokens;
+                if (columns <= 4) {
+                    launch(mask, std::integral_constant<int, 4>{});
+                } else if (columns <= 8) {
+                    launch(mask, std::integral_constant<int, 8>{});
+                } else {
+                    launch(mask, std::integral_constant<int, 16>{});
                 }
             });
             if (rc != OK) {
