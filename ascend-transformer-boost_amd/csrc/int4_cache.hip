@@ -31,6 +31,60 @@ struct WriteArgs {
     int32_t blockSize;
 };
 
+struct RowCodes {
+    uint32_t codes; // of the lane's eight values
+    RowParams params;
+};
+
+template <int CTRL> __device__ __forceinline__ float Moved(float x)
+{
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+
+// Maximum of hi and minimum of lo over LPR neighbouring lanes.
+template <int LPR> __device__ __forceinline__ void RowSpan(float &hi, float &lo)
+{
+    hi = fmaxf(hi, Moved<0xb1>(hi)); // lanes 1, 0, 3, 2 of four
+    lo = fminf(lo, Moved<0xb1>(lo));
+    hi = fmaxf(hi, Moved<0x4e>(hi)); // lanes 2, 3, 0, 1
+    lo = fminf(lo, Moved<0x4e>(lo));
+    hi = fmaxf(hi, Moved<0x141>(hi)); // eight lanes in reverse
+    lo = fminf(lo, Moved<0x141>(lo));
+    if constexpr (LPR >= 16) {
+        hi = fmaxf(hi, Moved<0x140>(hi)); // sixteen lanes in reverse
+        lo = fminf(lo, Moved<0x140>(lo));
+    }
+    if constexpr (LPR == 32) {
+        hi = fmaxf(hi, __shfl_xor(hi, 16));
+        lo = fminf(lo, __shfl_xor(lo, 16));
+    }
+}
+
+// Quantises a row that LPR lanes hold, eight values each.
+template <int LPR, bool BF16> __device__ __forceinline__ RowCodes CodesOf(const u32x4 w)
+{
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = Widen<BF16>(static_cast<uint16_t>(w[i]));
+        x[2 * i + 1] = Widen<BF16>(static_cast<uint16_t>(w[i] >> 16));
+    }
+    float hi = x[0], lo = x[0];
+    float none = 0.0f; // NaN if a value is infinite or NaN
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        hi = fmaxf(hi, x[i]);
+        lo = fminf(lo, x[i]);
+        none = __builtin_fmaf(x[i], 0.0f, none);
+    }
+    hi = none == 0.0f ? hi : INFINITY;
+    RowSpan<LPR>(hi, lo);
+    RowCodes r;
+    r.params = ParamsOf<BF16>(hi, lo, hi == INFINITY);
+    r.codes = Codes8(x, r.params);
+    return r;
+}
+
 // One row (token, head) to D / 8 lanes; blockIdx.y: 0 keys, 1 values.
 template <int D, bool BF16, bool VEC>
 __global__ __launch_bounds__(MOVE_THREADS) void WriteKernel(const WriteArgs a)
@@ -45,58 +99,116 @@ __global__ __launch_bounds__(MOVE_THREADS) void WriteKernel(const WriteArgs a)
     const int64_t slot = live ? a.slots[token] : -1;
     const uint16_t *src = isValue ? a.value + token * a.valueTokenStride : a.key + token * a.keyTokenStride;
     src += g * D + l * 8;
-    float x[8];
+    u32x4 w;
     if constexpr (VEC) {
-        const u32x4 w = *reinterpret_cast<const u32x4 *>(src);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = Widen<BF16>(static_cast<uint16_t>(w[i]));
-            x[2 * i + 1] = Widen<BF16>(static_cast<uint16_t>(w[i] >> 16));
-        }
+        w = *reinterpret_cast<const u32x4 *>(src);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            x[i] = Widen<BF16>(src[i]);
+        for (int i = 0; i < 4; ++i) {
+            w[i] = src[2 * i] | (static_cast<uint32_t>(src[2 * i + 1]) << 16);
         }
     }
-    float hi = x[0], lo = x[0];
-    bool finite = true;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        hi = fmaxf(hi, x[i]);
-        lo = fminf(lo, x[i]);
-        finite = finite && __builtin_isfinite(x[i]);
-    }
-    float bad = finite ? 0.0f : 1.0f;
-#pragma unroll
-    for (int step = 1; step < LPR; step *= 2) {
-        hi = fmaxf(hi, __shfl_xor(hi, step));
-        lo = fminf(lo, __shfl_xor(lo, step));
-        bad = fmaxf(bad, __shfl_xor(bad, step));
-    }
+    const RowCodes r = CodesOf<LPR, BF16>(w);
     if (slot < 0 || slot >= a.numSlots) {
         return; // (after the last cross-lane step)
     }
-    const RowParams p = ParamsOf<BF16>(hi, lo, bad != 0.0f);
-    uint32_t codes = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        codes |= CodeOf(x[i], p) << (4 * i);
-    }
-    const int64_t block = slot / a.blockSize;
+    const int64_t block = static_cast<int32_t>(slot) / a.blockSize;
     const int at = static_cast<int>(slot - block * a.blockSize);
     const int64_t head = block * a.G + g;
     if (isValue) {
         uint8_t *dst = a.valueCache + (head * (D / 2) + l * 4) * a.blockSize + at;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            dst[static_cast<int64_t>(i) * a.blockSize] = static_cast<uint8_t>(codes >> (8 * i));
+            dst[static_cast<int64_t>(i) * a.blockSize] = static_cast<uint8_t>(r.codes >> (8 * i));
         }
     } else {
-        *reinterpret_cast<uint32_t *>(a.keyCache + (head * a.blockSize + at) * (D / 2) + l * 4) = codes;
+        *reinterpret_cast<uint32_t *>(a.keyCache + (head * a.blockSize + at) * (D / 2) + l * 4) = r.codes;
     }
     if (l == 0) {
-        (isValue ? a.valueParams : a.keyParams)[head * a.blockSize + at] = p.word;
+        (isValue ? a.valueParams : a.keyParams)[head * a.blockSize + at] = r.params.word;
+    }
+}
+
+// The same for many tokens: a workgroup takes 64 tokens of one head, a wave 16 of them. Value codes lie token after token in
+// the cache, so they are turned in LDS: a wave then stores 64 neighbouring tokens' bytes of one channel pair at a time,
+// which the memory takes as one piece where the tokens' slots follow each other (as a prompt's do) and byte by byte where
+// they do not. (2048 new tokens of 5 sequences with 8 heads of 128 channels: 40 -> 21 us, against bytes stored from
+// the lanes of the row; one token a call of 512 sequences: 7 us in rows, 11 us in tiles, so that fewer than 1024 go in rows.)
+constexpr int TILE_TOKENS = 64;
+constexpr int TILE_FROM = 1024;
+template <int D, bool BF16, bool VEC>
+__global__ __launch_bounds__(MOVE_THREADS) void WriteTileKernel(const WriteArgs a)
+{
+    constexpr int LPR = D / 8;
+    constexpr int ROWS = WAVE / LPR;    // rows a wave works on at once
+    constexpr int STEPS = 16 / ROWS;
+    constexpr int PITCH = TILE_TOKENS + 4;
+    __shared__ uint8_t turned[D / 2][PITCH];
+    __shared__ uint32_t params[TILE_TOKENS];
+    const bool isValue = blockIdx.y != 0;
+    const int64_t tile = blockIdx.x / a.G;
+    const int g = static_cast<int>(blockIdx.x - tile * a.G);
+    const int lane = threadIdx.x & (WAVE - 1);
+    const int wave = threadIdx.x / WAVE;
+    const int l = lane % LPR;
+    const int64_t token0 = tile * TILE_TOKENS;
+    const int tokens = static_cast<int>(min(static_cast<int64_t>(TILE_TOKENS), a.numRows / a.G - token0));
+    const uint16_t *src = (isValue ? a.value : a.key) + g * D + l * 8;
+    const int64_t stride = isValue ? a.valueTokenStride : a.keyTokenStride;
+    u32x4 w[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        const uint16_t *from = src + (token0 + min(wave * 16 + s * ROWS + lane / LPR, tokens - 1)) * stride;
+        if constexpr (VEC) {
+            w[s] = *reinterpret_cast<const u32x4 *>(from);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[s][i] = from[2 * i] | (static_cast<uint32_t>(from[2 * i + 1]) << 16);
+            }
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        const int t = wave * 16 + s * ROWS + lane / LPR; // (past the last token: the last one again, not stored)
+        const RowCodes row = CodesOf<LPR, BF16>(w[s]);
+        if (isValue) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                turned[4 * l + i][t] = static_cast<uint8_t>(row.codes >> (8 * i));
+            }
+            if (l == 0) {
+                params[t] = row.params.word;
+            }
+        } else if (t < tokens) {
+            const int64_t slot = a.slots[token0 + t];
+            if (slot >= 0 && slot < a.numSlots) {
+                const int64_t block = static_cast<int32_t>(slot) / a.blockSize;
+                const int64_t at = (block * a.G + g) * a.blockSize + (slot - block * a.blockSize);
+                *reinterpret_cast<uint32_t *>(a.keyCache + at * (D / 2) + l * 4) = row.codes;
+                if (l == 0) {
+                    a.keyParams[at] = row.params.word;
+                }
+            }
+        }
+    }
+    if (!isValue) { // (the same for the whole workgroup)
+        return;
+    }
+    __syncthreads();
+    const int64_t slot = lane < tokens ? a.slots[token0 + lane] : -1;
+    if (slot < 0 || slot >= a.numSlots) {
+        return;
+    }
+    const int64_t block = static_cast<int32_t>(slot) / a.blockSize;
+    const int at = static_cast<int>(slot - block * a.blockSize);
+    const int64_t head = block * a.G + g;
+    uint8_t *dst = a.valueCache + head * (D / 2) * a.blockSize + at;
+    for (int pair = wave; pair < D / 2; pair += MOVE_THREADS / WAVE) {
+        dst[static_cast<int64_t>(pair) * a.blockSize] = turned[pair][lane];
+    }
+    if (wave == 0) {
+        a.valueParams[head * a.blockSize + at] = params[lane];
     }
 }
 
@@ -145,72 +257,83 @@ template <bool BF16> __device__ __forceinline__ u32x4 Expand(uint32_t codes, flo
     return out;
 }
 
-// A wave takes 16 x (64 / (D / 8)) positions of one sequence and head, counted from the 16-token group that holds the
-// sequence's first one: lane (l, grp) owns channels 8 l .. 8 l + 7 of the 16 positions of its group, which lie in one
-// block. Value codes lie token after token, so the lane reads four 16-byte runs (its four channel pairs) and turns
-// them by 4 x 4 byte transpositions; no shared memory.
+// A wave takes the keys or the values of 16 x (64 / (D / 8)) positions of one sequence and head, counted from the 16-token
+// group that holds the sequence's first one: lane (l, grp) owns channels 8 l .. 8 l + 7 of the 16 positions of its group,
+// which lie in one block. Everything is asked for before the first row is stored. Value codes lie token after token, so the
+// lane reads four 16-byte runs (its four channel pairs) and turns them by 4 x 4 byte transpositions; no shared memory. One
+// wave a workgroup: a short prefix is spread over as many CUs as it has pieces.
 template <int D, bool BF16>
-__global__ __launch_bounds__(MOVE_THREADS) void LoadKernel(const LoadArgs a)
+__global__ __launch_bounds__(WAVE) void LoadKernel(const LoadArgs a)
 {
     constexpr int LPR = D / 8;
     constexpr int GROUPS = WAVE / LPR;
-    const int lane = threadIdx.x & (WAVE - 1);
-    const int wave = threadIdx.x / WAVE;
+    const int lane = threadIdx.x;
+    const bool isValue = (blockIdx.x & 1) != 0;
     const int b = blockIdx.y;
     const int g = blockIdx.z;
     const int l = lane % LPR;
     const int start = a.starts ? max(a.starts[b], 0) : 0;
     const int len = min(a.lens[b], a.maxSeqLen);
-    const int64_t pos0 = (static_cast<int64_t>(start) & ~15LL) +
-                         ((static_cast<int64_t>(blockIdx.x) * (MOVE_THREADS / WAVE) + wave) * GROUPS + lane / LPR) * 16;
+    const int64_t pos0 = (static_cast<int64_t>(start) & ~15LL) + (static_cast<int64_t>(blockIdx.x / 2) * GROUPS + lane / LPR) * 16;
     const int64_t end = static_cast<int64_t>(start) + len;
+    if (__ballot(pos0 < end) == 0) {
+        return; // (before the sum below, which all lanes take part in)
+    }
     const int64_t rowsBefore = RowsBefore(a.lens, b, lane);
     if (pos0 >= end) {
         return;
     }
-    const int64_t tableAt = pos0 / a.blockSize;
-    if (tableAt >= a.maxBlocksPerSeq) {
+    if (pos0 >= static_cast<int64_t>(a.maxBlocksPerSeq) * a.blockSize) { // (that is below 2^30)
         return;
     }
+    const int tableAt = static_cast<int>(pos0) / a.blockSize;
     const int block = a.tables[static_cast<int64_t>(b) * a.maxBlocksPerSeq + tableAt];
     if (block < 0 || block >= a.numBlocks) {
         return;
     }
-    const int at = static_cast<int>(pos0 - tableAt * a.blockSize);
+    const int at = static_cast<int>(pos0) - tableAt * a.blockSize;
     const int64_t head = static_cast<int64_t>(block) * a.G + g;
     const int64_t firstRow = rowsBefore + pos0 - start; // row of the group's first position (below the sequence's own
                                                         // first row where the group begins in front of it)
-    const uint8_t *kc = a.keyCache + (head * a.blockSize + at) * (D / 2) + l * 4;
-    const uint32_t *kp = a.keyParams + head * a.blockSize + at;
-    const uint32_t *vp = a.valueParams + head * a.blockSize + at;
-    const uint8_t *vc = a.valueCache + (head * (D / 2) + l * 4) * a.blockSize + at;
-    u32x4 pairs[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        pairs[i] = *reinterpret_cast<const u32x4 *>(vc + static_cast<int64_t>(i) * a.blockSize);
-    }
+    const u32x4 *params = reinterpret_cast<const u32x4 *>((isValue ? a.valueParams : a.keyParams) + head * a.blockSize + at);
+    u32x4 param[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-        // tokens 4 q .. 4 q + 3: byte t of pairs[i][q] is pair i of token 4 q + t
-        const uint32_t lo01 = __builtin_amdgcn_perm(pairs[1][q], pairs[0][q], 0x05010400u); // t0: p0 p1, t1: p0 p1
-        const uint32_t lo23 = __builtin_amdgcn_perm(pairs[3][q], pairs[2][q], 0x05010400u);
-        const uint32_t hi01 = __builtin_amdgcn_perm(pairs[1][q], pairs[0][q], 0x07030602u);
-        const uint32_t hi23 = __builtin_amdgcn_perm(pairs[3][q], pairs[2][q], 0x07030602u);
-        const uint32_t codes[4] = {
-            __builtin_amdgcn_perm(lo23, lo01, 0x05040100u), __builtin_amdgcn_perm(lo23, lo01, 0x07060302u),
-            __builtin_amdgcn_perm(hi23, hi01, 0x05040100u), __builtin_amdgcn_perm(hi23, hi01, 0x07060302u)};
+        param[q] = params[q];
+    }
+    uint32_t codes[16];
+    if (isValue) {
+        const uint8_t *vc = a.valueCache + (head * (D / 2) + l * 4) * a.blockSize + at;
+        u32x4 pairs[4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const int j = 4 * q + t;
-            const int64_t row = firstRow + j;
-            if (pos0 + j >= start && pos0 + j < end && row < a.outRows) {
-                const int64_t dst = (row * a.G + g) * D + l * 8;
-                const uint32_t kw = kp[j];
-                const uint32_t vw = vp[j];
-                const uint32_t kcodes = *reinterpret_cast<const uint32_t *>(kc + static_cast<int64_t>(j) * (D / 2));
-                *reinterpret_cast<u32x4 *>(a.key + dst) = Expand<BF16>(kcodes, ScaleOf<BF16>(kw), MidOf<BF16>(kw));
-                *reinterpret_cast<u32x4 *>(a.value + dst) = Expand<BF16>(codes[t], ScaleOf<BF16>(vw), MidOf<BF16>(vw));
-            }
+        for (int i = 0; i < 4; ++i) {
+            pairs[i] = *reinterpret_cast<const u32x4 *>(vc + static_cast<int64_t>(i) * a.blockSize);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            // tokens 4 q .. 4 q + 3: byte t of pairs[i][q] is pair i of token 4 q + t
+            const uint32_t lo01 = __builtin_amdgcn_perm(pairs[1][q], pairs[0][q], 0x05010400u); // t0: p0 p1, t1: p0 p1
+            const uint32_t lo23 = __builtin_amdgcn_perm(pairs[3][q], pairs[2][q], 0x05010400u);
+            const uint32_t hi01 = __builtin_amdgcn_perm(pairs[1][q], pairs[0][q], 0x07030602u);
+            const uint32_t hi23 = __builtin_amdgcn_perm(pairs[3][q], pairs[2][q], 0x07030602u);
+            codes[4 * q] = __builtin_amdgcn_perm(lo23, lo01, 0x05040100u);
+            codes[4 * q + 1] = __builtin_amdgcn_perm(lo23, lo01, 0x07060302u);
+            codes[4 * q + 2] = __builtin_amdgcn_perm(hi23, hi01, 0x05040100u);
+            codes[4 * q + 3] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302u);
+        }
+    } else {
+        const uint8_t *kc = a.keyCache + (head * a.blockSize + at) * (D / 2) + l * 4;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            codes[j] = *reinterpret_cast<const uint32_t *>(kc + j * (D / 2));
+        }
+    }
+    u32x4 *out = reinterpret_cast<u32x4 *>((isValue ? a.value : a.key) + (firstRow * a.G + g) * D + l * 8);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        if (pos0 + j >= start && pos0 + j < end && firstRow + j < a.outRows) {
+            const uint32_t word = param[j / 4][j % 4];
+            out[static_cast<int64_t>(j) * a.G * (D / 8)] = Expand<BF16>(codes[j], ScaleOf<BF16>(word), MidOf<BF16>(word));
         }
     }
 }
@@ -264,8 +387,10 @@ extern "C" int atbmi_reshape_and_cache_int4(const void *key, const void *value, 
     a.G = static_cast<int32_t>(numKvHeads);
     a.blockSize = static_cast<int32_t>(blockSize);
     const bool vec = int4kv::Aligned16(key) && int4kv::Aligned16(value) && keyTokenStride % 8 == 0 && valueTokenStride % 8 == 0;
+    const bool tiles = numTokens >= int4kv::TILE_FROM;
     const int64_t rowsPerWg = int4kv::MOVE_THREADS / (headDim / 8);
-    const int64_t groups = (a.numRows + rowsPerWg - 1) / rowsPerWg;
+    const int64_t groups = tiles ? (numTokens + int4kv::TILE_TOKENS - 1) / int4kv::TILE_TOKENS * numKvHeads
+                                 : (a.numRows + rowsPerWg - 1) / rowsPerWg;
     if (groups > 0x7fffffffLL) {
         return Fail(ERR_INVALID_PARAM, "reshape_and_cache_int4: %lld rows are more than one launch takes",
                     (long long)a.numRows);
@@ -275,8 +400,13 @@ extern "C" int atbmi_reshape_and_cache_int4(const void *key, const void *value, 
     int4kv::WithHeadDim(headDim, [&](auto d) {
         int4kv::WithFlag(dtype == ATBMI_BF16, [&](auto bf16) {
             int4kv::WithFlag(vec, [&](auto v) {
-                int4kv::WriteKernel<decltype(d)::value, decltype(bf16)::value, decltype(v)::value>
-                    <<<grid, int4kv::MOVE_THREADS, 0, s>>>(a);
+                constexpr int D = decltype(d)::value;
+                constexpr bool BF16 = decltype(bf16)::value, VEC = decltype(v)::value;
+                if (tiles) {
+                    int4kv::WriteTileKernel<D, BF16, VEC><<<grid, int4kv::MOVE_THREADS, 0, s>>>(a);
+                } else {
+                    int4kv::WriteKernel<D, BF16, VEC><<<grid, int4kv::MOVE_THREADS, 0, s>>>(a);
+                }
             });
         });
     });
@@ -313,7 +443,7 @@ extern "C" int atbmi_paged_cache_load_int4(const uint8_t *keyCache, const uint8_
     }
     // (no sequence is longer than the table's reach)
     const int64_t longest = maxSeqLen < maxBlocksPerSeq * blockSize ? maxSeqLen : maxBlocksPerSeq * blockSize;
-    const int64_t perWg = 16LL * (int4kv::MOVE_THREADS / (headDim / 8));
+    const int64_t perWg = 16LL * (WAVE / (headDim / 8));
     const int64_t chunks = (longest + 15 + perWg - 1) / perWg; // (a sequence may begin 15 places into its first group)
     if (batch > 65535 || numKvHeads > 65535) {
         return Fail(ERR_INVALID_PARAM, "paged_cache_load_int4: %lld sequences with %lld heads are more than one launch takes",
@@ -335,11 +465,11 @@ extern "C" int atbmi_paged_cache_load_int4(const uint8_t *keyCache, const uint8_
     a.numBlocks = static_cast<int32_t>(numBlocks);
     a.G = static_cast<int32_t>(numKvHeads);
     a.maxSeqLen = static_cast<int32_t>(longest);
-    const dim3 grid(static_cast<unsigned>(chunks), static_cast<unsigned>(batch), static_cast<unsigned>(numKvHeads));
+    const dim3 grid(static_cast<unsigned>(2 * chunks), static_cast<unsigned>(batch), static_cast<unsigned>(numKvHeads));
     hipStream_t s = static_cast<hipStream_t>(stream);
     int4kv::WithHeadDim(headDim, [&](auto d) {
         int4kv::WithFlag(dtype == ATBMI_BF16, [&](auto bf16) {
-            int4kv::LoadKernel<decltype(d)::value, decltype(bf16)::value><<<grid, int4kv::MOVE_THREADS, 0, s>>>(a);
+            int4kv::LoadKernel<decltype(d)::value, decltype(bf16)::value><<<grid, WAVE, 0, s>>>(a);
         });
     });
     ATBMI_HIP_CHECK(hipGetLastError());

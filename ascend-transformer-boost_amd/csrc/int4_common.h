@@ -56,16 +56,24 @@ template <bool BF16> __device__ __forceinline__ RowParams ParamsOf(float hi, flo
     return p;
 }
 
-// rint((x - mid) / scale + 7.5) in 0 .. 15; 8 where the scale is 0 or the row is not finite (x is then ignored). All
-// three numbers have few bits, so whole quotients, which the half makes ties, are common: the product with 1 / scale is
-// corrected by its remainder, which makes them exact, and ties go to the even code as the definition has it.
-__device__ __forceinline__ uint32_t CodeOf(float x, const RowParams &p)
+// Codes of eight values, the first in the lowest four bits: rint((x - mid) / scale + 7.5) in 0 .. 15; 8 where the scale is
+// 0 or the row is not finite (x is then ignored). All three numbers have few bits, so whole quotients, which the half makes
+// ties, are common: the product with 1 / scale is corrected by its remainder, which makes them exact, and ties go to the
+// even code as the definition has it. A sum with 1.5 2^23 is rounded to a whole number, which its lowest bits then are.
+__device__ __forceinline__ uint32_t Codes8(const float (&x)[8], const RowParams &p)
 {
-    const float d = x - p.mid;
-    const float q0 = d * p.inv;
-    const float quotient = __builtin_fmaf(__builtin_fmaf(-q0, p.scale, d), p.inv, q0);
-    const float q = p.inv == 0.0f ? 8.0f : rintf(quotient + 7.5f);
-    return static_cast<uint32_t>(fminf(fmaxf(q, 0.0f), 15.0f));
+    constexpr float MAGIC = 12582912.0f;
+    uint32_t codes = 0, extra = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float d = x[i] - p.mid;
+        const float q0 = d * p.inv;
+        const float quotient = __builtin_fmaf(__builtin_fmaf(-q0, p.scale, d), p.inv, q0);
+        const float q = __builtin_amdgcn_fmed3f(quotient + 7.5f, 0.0f, 15.0f) + MAGIC;
+        codes += __float_as_uint(q) << (4 * i);
+        extra += 0x4b400000u << (4 * i); // the bits of MAGIC
+    }
+    return p.inv == 0.0f ? 0x88888888u : codes - extra;
 }
 
 inline int CheckCache(const char *who, int32_t dtype, int64_t numKvHeads, int64_t headDim, int64_t blockSize,
