@@ -18,7 +18,7 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 _LIB = os.environ.get("ATB_MI_LIB_DIR") or os.path.join(_PKG, "lib")
 
 # aclDataType / aclFormat values (include/acl/acl.h)
-ACL_FLOAT, ACL_FLOAT16, ACL_INT8, ACL_INT32, ACL_INT64, ACL_BF16 = 0, 1, 2, 3, 9, 27
+ACL_FLOAT, ACL_FLOAT16, ACL_INT8, ACL_INT32, ACL_UINT8, ACL_INT64, ACL_BF16 = 0, 1, 2, 3, 4, 9, 27
 ACL_FORMAT_ND, ACL_FORMAT_FRACTAL_NZ = 2, 29
 ACL_DTYPE_BY_NAME = {
     "float": 0, "float16": 1, "int8": 2, "int32": 3, "uint8": 4, "int16": 6, "uint16": 7, "uint32": 8,
@@ -170,6 +170,39 @@ class MultiLatentAttentionParam(ctypes.Structure):
             if not hasattr(self, k):
                 raise AttributeError("MultiLatentAttentionParam has no field " + k)
             setattr(self, k, v)
+
+
+def _param(name, fields, size, doc, **defaults):
+    """Byte image of an atb::infer param with reserved bytes at its end."""
+    def init(self, **kw):
+        ctypes.Structure.__init__(self)
+        for k, v in {**defaults, **kw}.items():
+            if not hasattr(self, k):
+                raise AttributeError("%s has no field %s" % (name, k))
+            setattr(self, k, v)
+
+    used = 0
+    for _, t in fields:
+        used = (used + ctypes.sizeof(t) - 1) // ctypes.sizeof(t) * ctypes.sizeof(t) + ctypes.sizeof(t)
+    made = type(name, (ctypes.Structure,), {"__doc__": doc, "__init__": init,
+                                            "_fields_": fields + [("rsv", ctypes.c_uint8 * (size - used))]})
+    assert ctypes.sizeof(made) == size
+    return made
+
+
+RmsNormQuantParam = _param("RmsNormQuantParam", [("epsilon", ctypes.c_float), ("hasResidual", ctypes.c_bool)], 16,
+                           "Byte image of atb::infer::RmsNormQuantParam (16 bytes).", epsilon=1e-5)
+LinearInt8Param = _param("LinearInt8Param", [("outDataType", ctypes.c_int32), ("hasBias", ctypes.c_bool)], 16,
+                         "Byte image of atb::infer::LinearInt8Param (16 bytes).", outDataType=ACL_FLOAT16)
+ReshapeAndCacheInt4Param = _param("ReshapeAndCacheInt4Param", [], 16,
+                                  "Byte image of atb::infer::ReshapeAndCacheInt4Param (16 bytes).")
+PagedCacheLoadInt4Param = _param("PagedCacheLoadInt4Param", [("hasSeqStarts", ctypes.c_bool)], 16,
+                                 "Byte image of atb::infer::PagedCacheLoadInt4Param (16 bytes).")
+PagedAttentionInt4Param = _param(
+    "PagedAttentionInt4Param",
+    [("headNum", ctypes.c_int32), ("kvHeadNum", ctypes.c_int32), ("qkScale", ctypes.c_float),
+     ("queryTokens", ctypes.c_int32), ("hasMask", ctypes.c_bool)], 32,
+    "Byte image of atb::infer::PagedAttentionInt4Param (32 bytes).", qkScale=1.0, queryTokens=1)
 
 
 class AtbmiPaShape(ctypes.Structure):
@@ -421,7 +454,7 @@ def make_tensor(dtype, shape, device_ptr=None, host_ptr=None, fmt=ACL_FORMAT_ND,
 def _torch_acl_dtype(t):
     import torch
     return {torch.float16: ACL_FLOAT16, torch.bfloat16: ACL_BF16, torch.int8: ACL_INT8, torch.int32: ACL_INT32,
-            torch.float32: ACL_FLOAT, torch.int64: ACL_INT64}[t.dtype]
+            torch.float32: ACL_FLOAT, torch.int64: ACL_INT64, torch.uint8: ACL_UINT8}[t.dtype]
 
 
 def tensor_of(t, host=None):

@@ -151,6 +151,31 @@ int32_t atb_c_create_operation(const char *opName, const void *param, uint64_t p
         memcpy(static_cast<void *>(&p), param, sizeof(p));
         return atb::CreateOperation(p, out);
     }
+    if (!strcmp(opName, "RmsNormQuantOperation") && paramSize == sizeof(atb::infer::RmsNormQuantParam)) {
+        atb::infer::RmsNormQuantParam p;
+        memcpy(static_cast<void *>(&p), param, sizeof(p));
+        return atb::CreateOperation(p, out);
+    }
+    if (!strcmp(opName, "LinearInt8Operation") && paramSize == sizeof(atb::infer::LinearInt8Param)) {
+        atb::infer::LinearInt8Param p;
+        memcpy(static_cast<void *>(&p), param, sizeof(p));
+        return atb::CreateOperation(p, out);
+    }
+    if (!strcmp(opName, "ReshapeAndCacheInt4Operation") && paramSize == sizeof(atb::infer::ReshapeAndCacheInt4Param)) {
+        atb::infer::ReshapeAndCacheInt4Param p;
+        memcpy(static_cast<void *>(&p), param, sizeof(p));
+        return atb::CreateOperation(p, out);
+    }
+    if (!strcmp(opName, "PagedCacheLoadInt4Operation") && paramSize == sizeof(atb::infer::PagedCacheLoadInt4Param)) {
+        atb::infer::PagedCacheLoadInt4Param p;
+        memcpy(static_cast<void *>(&p), param, sizeof(p));
+        return atb::CreateOperation(p, out);
+    }
+    if (!strcmp(opName, "PagedAttentionInt4Operation") && paramSize == sizeof(atb::infer::PagedAttentionInt4Param)) {
+        atb::infer::PagedAttentionInt4Param p;
+        memcpy(static_cast<void *>(&p), param, sizeof(p));
+        return atb::CreateOperation(p, out);
+    }
     return atb::ERROR_INVALID_PARAM;
 }
 

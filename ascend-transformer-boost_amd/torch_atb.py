@@ -18,7 +18,9 @@ whose outputs are their inputs updated in place (ReshapeAndCache, NormRopeReshap
 tensors instead of fresh ones. ReshapeAndCacheWithStrideParam, ReshapeAndCacheOmniParam, NormRopeReshapeParam,
 MultiLatentAttentionParam, BlockCopyParam and PagedCacheLoadParam are not bound by the reference's module; they are offered here in the same style
 (for ReshapeAndCacheWithStride, key / value are [tokens, heads, head_size] tensors that start at the base
-of the storage which the strides and the offset index into).
+of the storage which the strides and the offset index into). RmsNormQuantParam, LinearInt8Param, ReshapeAndCacheInt4Param,
+PagedCacheLoadInt4Param and PagedAttentionInt4Param (8-bit activations and weights, a 4-bit cache) are this library's own;
+the `quantized` module offers the same operators as functions that do not wait for the device.
 """
 import enum
 import re
@@ -185,6 +187,31 @@ class PagedCacheLoadParam(_Param):
         K_CACHE_V_CACHE_ND = 1
 
 
+class RmsNormQuantParam(_Param):
+    _struct = _b.RmsNormQuantParam
+    _op_name = "RmsNormQuantOperation"
+
+
+class LinearInt8Param(_Param):
+    _struct = _b.LinearInt8Param
+    _op_name = "LinearInt8Operation"
+
+
+class ReshapeAndCacheInt4Param(_Param):
+    _struct = _b.ReshapeAndCacheInt4Param
+    _op_name = "ReshapeAndCacheInt4Operation"
+
+
+class PagedCacheLoadInt4Param(_Param):
+    _struct = _b.PagedCacheLoadInt4Param
+    _op_name = "PagedCacheLoadInt4Operation"
+
+
+class PagedAttentionInt4Param(_Param):
+    _struct = _b.PagedAttentionInt4Param
+    _op_name = "PagedAttentionInt4Operation"
+
+
 # operation name -> indices of the inputs that its outputs are (updated in place), by input count
 _IN_PLACE = {
     "ReshapeAndCacheOperation": {5: [2, 3], 3: [1], 7: [2, 3], 8: [2, 3]},  # 7 / 8: head compression
@@ -192,6 +219,8 @@ _IN_PLACE = {
     "ReshapeAndCacheOmniOperation": {8: [2, 3]},
     "NormRopeReshapeOperation": {7: [6]},
     "PagedCacheLoadOperation": {7: [4, 5]},
+    "ReshapeAndCacheInt4Operation": {7: [2, 3, 4, 5]},
+    "PagedCacheLoadInt4Operation": {8: [6, 7], 9: [6, 7]},
 }
 
 
@@ -250,7 +279,8 @@ class Operation:
             st, descs = self._op.infer_shape(ins)
             if st != 0:
                 raise RuntimeError("call operation_->InferShape fail: %s" % _b.ERROR_NAMES[st])
-            rev = {_b.ACL_FLOAT16: torch.float16, _b.ACL_BF16: torch.bfloat16, _b.ACL_INT8: torch.int8}
+            rev = {_b.ACL_FLOAT16: torch.float16, _b.ACL_BF16: torch.bfloat16, _b.ACL_INT8: torch.int8,
+                   _b.ACL_FLOAT: torch.float32}
             outputs = [torch.empty([d.dims[i] for i in range(d.dimNum)], dtype=rev[d.dtype], device=device)
                        for d in descs]
         outs = [_b.tensor_of(t) for t in outputs]

@@ -257,6 +257,58 @@ struct PagedCacheLoadParam {
     uint8_t rsv[61] = {0};            // must stay zero
 };
 
+// The next five make up the attention half of a decoder layer with 8-bit activations and weights and a paged KV cache in
+// 4 bits; include/atbmi_kernels.h defines their arithmetic and the cache's layout. The cache is four tensors: keyCache
+// uint8 [blocks, kvHeads, blockSize, headSize / 2], valueCache uint8 [blocks, kvHeads, headSize / 2, blockSize], keyParams
+// and valueParams [blocks, kvHeads, blockSize, 2] in the model's type (float16 or bf16).
+
+// RMS norm of rows (with a residual: of the rounded sum) to int8 with a scale for each row. Inputs: x [rows, dim], gamma
+// [dim], [residual [rows, dim]]; outputs: int8 [rows, dim], float [rows], [the sum [rows, dim]].
+struct RmsNormQuantParam {
+    float epsilon = 1e-5;     // added to the mean square; finite, not below 0
+    bool hasResidual = false; // a residual is added first, and the sum is an output
+    uint8_t rsv[11] = {0};    // must stay zero
+};
+
+// Product of int8 rows and int8 weights with a scale for each row of both. Inputs: x int8 [m, k], weight int8 [n, k],
+// xScale float [m], weightScale float [n], [bias float [n]]; output [m, n].
+struct LinearInt8Param {
+    aclDataType outDataType = ACL_FLOAT16; // ACL_FLOAT16 or ACL_BF16
+    bool hasBias = false;
+    uint8_t rsv[11] = {0}; // must stay zero
+};
+
+// Quantises new key and value rows into the 4-bit cache. Inputs: key, value [tokens, kvHeads, headSize], the cache's four
+// tensors, slotMapping int32 [tokens]; the outputs are the cache's tensors, updated in place.
+struct ReshapeAndCacheInt4Param {
+    uint8_t rsv[16] = {0}; // must stay zero
+};
+
+// Gathers the rows of every sequence from the 4-bit cache. Inputs: the cache's four tensors, blockTables int32 [batch,
+// maxBlocks], seqLens int32 [batch], key, value [tokens, kvHeads, headSize], [seqStarts int32 [batch]]; the outputs are key
+// and value, updated in place.
+struct PagedCacheLoadInt4Param {
+    bool hasSeqStarts = false; // seqStarts gives the first cached position of every sequence
+    uint8_t rsv[15] = {0};     // must stay zero
+};
+
+// Decode attention over the 4-bit cache. Inputs: query [batch * queryTokens, headNum, headSize], the cache's four tensors,
+// blockTables int32 [batch, maxBlocks], contextLens int32 [batch], [mask [batch | 1, headNum | 1, queryTokens | 1,
+// positions]]; output like query. The lengths stay on the device.
+struct PagedAttentionInt4Param {
+    int32_t headNum = 0;
+    int32_t kvHeadNum = 0;   // divides headNum
+    float qkScale = 1.0;     // finite, above 0
+    int32_t queryTokens = 1; // 1 .. 64; token j of a sequence sees its first contextLens - queryTokens + 1 + j positions
+    bool hasMask = false;
+    uint8_t rsv[15] = {0};   // must stay zero
+};
+
+static_assert(sizeof(RmsNormQuantParam) == 16, "RmsNormQuantParam ABI size");
+static_assert(sizeof(LinearInt8Param) == 16, "LinearInt8Param ABI size");
+static_assert(sizeof(ReshapeAndCacheInt4Param) == 16, "ReshapeAndCacheInt4Param ABI size");
+static_assert(sizeof(PagedCacheLoadInt4Param) == 16, "PagedCacheLoadInt4Param ABI size");
+static_assert(sizeof(PagedAttentionInt4Param) == 32, "PagedAttentionInt4Param ABI size");
 static_assert(sizeof(ReshapeAndCacheParam) == 24, "ReshapeAndCacheParam ABI size");
 static_assert(sizeof(ReshapeAndCacheWithStrideParam) == 24, "ReshapeAndCacheWithStrideParam ABI size");
 static_assert(sizeof(ReshapeAndCacheOmniParam) == 8, "ReshapeAndCacheOmniParam ABI size");

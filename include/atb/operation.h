@@ -35,7 +35,8 @@ public:
 };
 
 // Specialised for infer::PagedAttentionParam, ReshapeAndCacheParam, ReshapeAndCacheWithStrideParam,
-// ReshapeAndCacheOmniParam, RopeParam, ElewiseParam, NormRopeReshapeParam, MultiLatentAttentionParam, BlockCopyParam and PagedCacheLoadParam.
+// ReshapeAndCacheOmniParam, RopeParam, ElewiseParam, NormRopeReshapeParam, MultiLatentAttentionParam, BlockCopyParam, PagedCacheLoadParam,
+// RmsNormQuantParam, LinearInt8Param, ReshapeAndCacheInt4Param, PagedCacheLoadInt4Param and PagedAttentionInt4Param.
 template <typename OpParam> Status CreateOperation(const OpParam &opParam, Operation **operation);
 
 Status DestroyOperation(Operation *operation);

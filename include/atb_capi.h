@@ -42,11 +42,13 @@ int32_t atb_c_destroy_context(void *context);
 
 /* atb::CreateOperation for infer::PagedAttentionParam, ReshapeAndCacheParam,
  * ReshapeAndCacheWithStrideParam, ReshapeAndCacheOmniParam, RopeParam, ElewiseParam, NormRopeReshapeParam,
- * MultiLatentAttentionParam, BlockCopyParam and PagedCacheLoadParam. opName is the operation's name
+ * MultiLatentAttentionParam, BlockCopyParam, PagedCacheLoadParam, RmsNormQuantParam, LinearInt8Param,
+ * ReshapeAndCacheInt4Param, PagedCacheLoadInt4Param and PagedAttentionInt4Param. opName is the operation's name
  * ("PagedAttentionOperation", "ReshapeAndCacheOperation", "ReshapeAndCacheWithStrideOperation",
  * "ReshapeAndCacheOmniOperation", "RopeOperation", "ElewiseOperation", "NormRopeReshapeOperation",
- * "MultiLatentAttentionOperation", "BlockCopyOperation", "PagedCacheLoadOperation"); param points at the bytes of
- * the matching C++ param struct (120 / 24 / 24 / 8 / 16 / 64 / 28 / 64 / 16 / 64 bytes). */
+ * "MultiLatentAttentionOperation", "BlockCopyOperation", "PagedCacheLoadOperation", "RmsNormQuantOperation",
+ * "LinearInt8Operation", "ReshapeAndCacheInt4Operation", "PagedCacheLoadInt4Operation", "PagedAttentionInt4Operation"); param points at the bytes of
+ * the matching C++ param struct (120 / 24 / 24 / 8 / 16 / 64 / 28 / 64 / 16 / 64 / 16 / 16 / 16 / 16 / 32 bytes). */
 int32_t atb_c_create_operation(const char *opName, const void *param, uint64_t paramSize, void **operation);
 /* atb::DestroyOperation. */
 int32_t atb_c_destroy_operation(void *operation);
