@@ -1,7 +1,8 @@
-"""Builds the two shared libraries of the package, in-tree:
+"""Builds the shared libraries of the package, in-tree:
 
   lib/libatbmi_kernels.so  HIP kernels + C ABI (hipcc, --offload-arch=gfx950)
   lib/libatb.so            atb::Operation layer + flat C view (g++), links the first
+  lib/quantized_ext.so     the calls of quantized.py on torch tensors (g++), links torch and the first
 
 hipcc cross-compiles gfx950 code objects without a GPU, so this runs anywhere
 the ROCm toolchain is installed. Usage: python3 build.py [--jobs N] [--sanitize]
@@ -81,6 +82,26 @@ def build_host():
     return target
 
 
+def build_torch_ext():
+    """The extension module behind quantized.py (host code only; torch's headers want to know the HIP platform)."""
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    os.makedirs(LIB, exist_ok=True)
+    target = os.path.join(LIB, "quantized_ext.so")
+    torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    flags = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-I" + INCLUDE, "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI]
+    for path in cpp_extension.include_paths() + ["/opt/rocm/include", sysconfig.get_paths()["include"]]:
+        flags += ["-isystem", path]
+    out = _run([CXX] + flags + ["-shared", "-o", target, os.path.join(PKG, "torch_ext", "quantized_ext.cpp"), "-L" + torch_lib,
+                                "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_hip", "-lc10", "-L" + LIB, "-latbmi_kernels",
+                                "-Wl,-rpath,$ORIGIN"])
+    if out.strip():
+        print(out)
+    return target
+
+
 def build_tools():
     """The stand-alone HBM streaming benchmark (an executable, not part of the libraries)."""
     os.makedirs(LIB, exist_ok=True)
@@ -91,7 +112,10 @@ def build_tools():
 
 
 def build_all(jobs=8):
-    return [build_kernels(jobs), build_host(), build_tools()]
+    with concurrent.futures.ThreadPoolExecutor(max_workers=2) as pool:
+        kernels = build_kernels(jobs)
+        ext = pool.submit(build_torch_ext)
+        return [kernels, build_host(), ext.result(), build_tools()]
 
 
 def sanitizer_runtime():
