@@ -55,6 +55,7 @@ constexpr int PA_THREADS = PA_WAVES * WAVE;
 constexpr int MERGE_MOST_THREADS = 1024;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int START = 4;        // see UnitsOf
+constexpr int WHOLE_TILES = 16; // see ShapeOf
 constexpr float STEP_UP = 8.0f; // how far (log2) a score may exceed the reference before that moves
 
 struct PaInt4Args {
@@ -88,6 +89,7 @@ struct PaInt4Args {
     int32_t groupsPerBlock; // blockSize / 16
     uint32_t groupsMagic;   // ceil(2^32 / groupsPerBlock): x / groupsPerBlock for x * groupsPerBlock < 2^32 (0 for 1)
     int32_t numBlocks;
+    int32_t whole;          // 1: range r is sequence r, nothing is cut
     int32_t ranges;
     float scale2; // qkScale log2(e)
 };
@@ -264,34 +266,37 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
     const int ct = pair % a.colTiles;
 
     // ---- where the range begins
-    int units = 0;
-    for (int b = lane; b < a.batch; b += WAVE) {
-        units += UnitsOf(ContextLen(a, b));
-    }
-    units = WaveSum(units);
-    const int live = LiveRanges(a.ranges, units);
-    if (range >= live) {
-        return;
-    }
-    const int begin = RangeBegin(range, units, live);
-    const int end = RangeBegin(range + 1, units, live);
-    int seq = 0, before = 0; // the sequence that holds unit `begin`, units of the sequences before it
-    for (int b0 = 0;; b0 += WAVE) {
-        const int own = b0 + lane < a.batch ? UnitsOf(ContextLen(a, b0 + lane)) : 0;
-        int upTo = own;
+    int begin = 0, end = 1; // (of a whole sequence: any, it ends after the first)
+    int seq = range, before = 0; // the sequence that holds unit `begin`, units of the sequences before it
+    if (a.whole == 0) {
+        int units = 0;
+        for (int b = lane; b < a.batch; b += WAVE) {
+            units += UnitsOf(ContextLen(a, b));
+        }
+        units = WaveSum(units);
+        const int live = LiveRanges(a.ranges, units);
+        if (range >= live) {
+            return;
+        }
+        begin = RangeBegin(range, units, live);
+        end = RangeBegin(range + 1, units, live);
+        for (int b0 = 0;; b0 += WAVE) {
+            const int own = b0 + lane < a.batch ? UnitsOf(ContextLen(a, b0 + lane)) : 0;
+            int upTo = own;
 #pragma unroll
-        for (int step = 1; step < WAVE; step *= 2) {
-            const int other = __shfl_up(upTo, step);
-            upTo += lane >= step ? other : 0;
+            for (int step = 1; step < WAVE; step *= 2) {
+                const int other = __shfl_up(upTo, step);
+                upTo += lane >= step ? other : 0;
+            }
+            const uint64_t past = __ballot(before + upTo > begin);
+            if (past != 0) { // (begin < units: some sequence holds it)
+                const int at = __builtin_ctzll(past);
+                seq = b0 + at;
+                before += __shfl(upTo - own, at);
+                break;
+            }
+            before += __shfl(upTo, WAVE - 1);
         }
-        const uint64_t past = __ballot(before + upTo > begin);
-        if (past != 0) { // (begin < units: some sequence holds it)
-            const int at = __builtin_ctzll(past);
-            seq = b0 + at;
-            before += __shfl(upTo - own, at);
-            break;
-        }
-        before += __shfl(upTo, WAVE - 1);
     }
     seq = __builtin_amdgcn_readfirstlane(seq);
     before = __builtin_amdgcn_readfirstlane(before);
@@ -323,7 +328,7 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
     for (;;) {
         const int len = UniformLen(a, seq);
         const int tBegin = max(max(begin - before, 0) - START, 0);
-        const int tEnd = max(min(end - before, UnitsOf(len)) - START, tBegin);
+        const int tEnd = a.whole != 0 ? TilesOf(len) : max(min(end - before, UnitsOf(len)) - START, tBegin);
         // (block ids are read through the scalar cache: not counted with the tiles on their way)
         const auto *table = Scalar(a.tables + static_cast<int64_t>(seq) * a.maxBlocksPerSeq);
 
@@ -895,6 +900,7 @@ struct PaInt4Shape {
     int colTiles = 1;
     int64_t pairs = 1;
     int64_t ranges = 1;
+    bool whole = false; // a workgroup takes whole sequences
     bool merge = false; // some sequence may be cut
     uint64_t partO = 0, partM = 0, partL = 0, bytes = 0;
 };
@@ -909,7 +915,16 @@ PaInt4Shape ShapeOf(const AtbmiPaInt4Call *c)
     const int64_t perCu = c->headDim == 256 ? 1 : 2; // workgroups a CU holds at once (registers)
     s.ranges = std::max<int64_t>(1, DeviceComputeUnits() * perCu / s.pairs);
     s.ranges = std::min<int64_t>(s.ranges, std::max<int64_t>(1, ((mostTiles + START) * c->batch + PA_WAVES - 1) / PA_WAVES));
-    s.merge = s.ranges > 1 && mostTiles > 1;
+    // Whole sequences to a workgroup need no second kernel and no search for where a range begins, and leave the balance to
+    // the order in which workgroups end: taken where no sequence can be long, and up to twice that where there is a
+    // workgroup for every CU. (32 query heads over 8 of 128 channels, lengths n / 4 .. n. 1 sequence of 512: 11.1 us cut,
+    // 7.7 whole; 1 of 1024: 12.0, 10.9; 64 up to 1024: 25.3, 18.3; 64 up to 2048: 33.1, 27.7; but 1 of 2048: 13.1, 17.9;
+    // 4 up to 4096: 15.9, 30.6; 64 up to 8192: 90, 104.)
+    s.whole = mostTiles <= WHOLE_TILES || (mostTiles <= 2 * WHOLE_TILES && s.pairs * c->batch >= DeviceComputeUnits());
+    if (s.whole) {
+        s.ranges = c->batch;
+    }
+    s.merge = s.ranges > 1 && !s.whole;
     if (s.merge) {
         const uint64_t rows = static_cast<uint64_t>(2 * s.ranges * s.pairs) * HT;
         auto align = [](uint64_t v) { return (v + 255) / 256 * 256; };
@@ -1004,6 +1019,7 @@ extern "C" int atbmi_pa_int4_decode(const AtbmiPaInt4Call *call, void *workspace
     a.groupsPerBlock = call->blockSize / 16;
     a.groupsMagic = magic(a.groupsPerBlock);
     a.numBlocks = call->numBlocks;
+    a.whole = shape.whole ? 1 : 0;
     a.ranges = static_cast<int32_t>(shape.ranges);
     a.scale2 = call->qkScale * int4kv::LOG2E;
     hipStream_t s = static_cast<hipStream_t>(stream);
