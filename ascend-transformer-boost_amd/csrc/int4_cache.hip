@@ -12,6 +12,7 @@ namespace atbmi {
 namespace int4kv {
 
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int MOVE_THREADS = 256;
 
@@ -31,56 +32,62 @@ struct WriteArgs {
     int32_t blockSize;
 };
 
+template <int CTRL> __device__ __forceinline__ s16x2 Moved(s16x2 x)
+{
+    return __builtin_bit_cast(s16x2, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+
+// 16-bit floats as integers of the same order and back (two at a time): the bits below the sign are turned over where it is
+// set. NaN with a sign lie below -infinity, those without one above infinity.
+__device__ __forceinline__ s16x2 Ordered(s16x2 x)
+{
+    return x ^ ((x >> 15) & 0x7fff);
+}
+__device__ __forceinline__ s16x2 Ordered(uint32_t word)
+{
+    return Ordered(__builtin_bit_cast(s16x2, word));
+}
+
 struct RowCodes {
     uint32_t codes; // of the lane's eight values
     RowParams params;
 };
 
-template <int CTRL> __device__ __forceinline__ float Moved(float x)
-{
-    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true));
-}
-
-// Maximum of hi and minimum of lo over LPR neighbouring lanes.
-template <int LPR> __device__ __forceinline__ void RowSpan(float &hi, float &lo)
-{
-    hi = fmaxf(hi, Moved<0xb1>(hi)); // lanes 1, 0, 3, 2 of four
-    lo = fminf(lo, Moved<0xb1>(lo));
-    hi = fmaxf(hi, Moved<0x4e>(hi)); // lanes 2, 3, 0, 1
-    lo = fminf(lo, Moved<0x4e>(lo));
-    hi = fmaxf(hi, Moved<0x141>(hi)); // eight lanes in reverse
-    lo = fminf(lo, Moved<0x141>(lo));
-    if constexpr (LPR >= 16) {
-        hi = fmaxf(hi, Moved<0x140>(hi)); // sixteen lanes in reverse
-        lo = fminf(lo, Moved<0x140>(lo));
-    }
-    if constexpr (LPR == 32) {
-        hi = fmaxf(hi, __shfl_xor(hi, 16));
-        lo = fminf(lo, __shfl_xor(lo, 16));
-    }
-}
-
-// Quantises a row that LPR lanes hold, eight values each.
+// Quantises a row that LPR lanes hold, eight values each (w: as they are read). Maximum and minimum are taken on the 16-bit
+// values as integers, two to an instruction, the minimum as the maximum of the complements in the other half of a word:
+// the kernel for many tokens was bound by its arithmetic, 208 instructions for eight values, half of them for this.
 template <int LPR, bool BF16> __device__ __forceinline__ RowCodes CodesOf(const u32x4 w)
 {
+    s16x2 hi = Ordered(w[0]), lo = hi;
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+        const s16x2 v = Ordered(w[i]);
+        hi = __builtin_elementwise_max(hi, v);
+        lo = __builtin_elementwise_min(lo, v);
+    }
+    lo = ~lo;
+    s16x2 span = __builtin_elementwise_max(s16x2{hi[0], lo[0]}, s16x2{hi[1], lo[1]}); // maximum, ~minimum
+    span = __builtin_elementwise_max(span, Moved<0xb1>(span));  // lanes 1, 0, 3, 2 of four
+    span = __builtin_elementwise_max(span, Moved<0x4e>(span));  // lanes 2, 3, 0, 1
+    span = __builtin_elementwise_max(span, Moved<0x141>(span)); // eight lanes in reverse
+    if constexpr (LPR >= 16) {
+        span = __builtin_elementwise_max(span, Moved<0x140>(span)); // sixteen lanes in reverse
+    }
+    if constexpr (LPR == 32) {
+        span = __builtin_elementwise_max(span, __builtin_bit_cast(s16x2, __shfl_xor(__builtin_bit_cast(int, span), 16)));
+    }
+    span[1] = ~span[1];
+    span = Ordered(span);
+    constexpr int INF = BF16 ? 0x7f80 : 0x7c00;
+    const bool bad = (span[0] & 0x7fff) >= INF || (span[1] & 0x7fff) >= INF; // an infinity or NaN somewhere in the row
     float x[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         x[2 * i] = Widen<BF16>(static_cast<uint16_t>(w[i]));
         x[2 * i + 1] = Widen<BF16>(static_cast<uint16_t>(w[i] >> 16));
     }
-    float hi = x[0], lo = x[0];
-    float none = 0.0f; // NaN if a value is infinite or NaN
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        hi = fmaxf(hi, x[i]);
-        lo = fminf(lo, x[i]);
-        none = __builtin_fmaf(x[i], 0.0f, none);
-    }
-    hi = none == 0.0f ? hi : INFINITY;
-    RowSpan<LPR>(hi, lo);
     RowCodes r;
-    r.params = ParamsOf<BF16>(hi, lo, hi == INFINITY);
+    r.params = ParamsOf<BF16>(Widen<BF16>(static_cast<uint16_t>(span[0])), Widen<BF16>(static_cast<uint16_t>(span[1])), bad);
     r.codes = Codes8(x, r.params);
     return r;
 }
@@ -252,7 +259,7 @@ template <bool BF16> __device__ __forceinline__ u32x4 Expand(uint32_t codes, flo
     for (int i = 0; i < 4; ++i) {
         const float even = __builtin_fmaf(static_cast<float>((codes >> (8 * i)) & 15u) - 7.5f, scale, mid);
         const float odd = __builtin_fmaf(static_cast<float>((codes >> (8 * i + 4)) & 15u) - 7.5f, scale, mid);
-        out[i] = static_cast<uint32_t>(Narrow<BF16>(even)) | (static_cast<uint32_t>(Narrow<BF16>(odd)) << 16);
+        out[i] = NarrowPair<BF16>(even, odd);
     }
     return out;
 }

@@ -16,6 +16,18 @@ template <bool BF16> __device__ __forceinline__ uint16_t Narrow(float v)
     return BF16 ? FloatToBf16(v) : FloatToHalfBits(v);
 }
 
+// Two values in one word, the first in its low half (one instruction for bf16).
+template <bool BF16> __device__ __forceinline__ uint32_t NarrowPair(float a, float b)
+{
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    if constexpr (BF16) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+    } else {
+        return static_cast<uint32_t>(FloatToHalfBits(a)) | (static_cast<uint32_t>(FloatToHalfBits(b)) << 16);
+    }
+}
+
 // A row's parameter word: scale in the low half, middle in the high half.
 template <bool BF16> __device__ __forceinline__ float ScaleOf(uint32_t word)
 {
@@ -40,8 +52,9 @@ struct RowParams {
 template <bool BF16> __device__ __forceinline__ RowParams ParamsOf(float hi, float lo, bool bad)
 {
     RowParams p;
-    uint16_t scale = Narrow<BF16>((0.5f * hi - 0.5f * lo) * (2.0f / 15.0f));
-    uint16_t mid = Narrow<BF16>(0.5f * hi + 0.5f * lo);
+    const uint32_t both = NarrowPair<BF16>((0.5f * hi - 0.5f * lo) * (2.0f / 15.0f), 0.5f * hi + 0.5f * lo);
+    uint16_t scale = static_cast<uint16_t>(both);
+    uint16_t mid = static_cast<uint16_t>(both >> 16);
     if (BF16 && (scale & 0x7f80u) == 0) {
         scale = 0;
     }
@@ -49,7 +62,7 @@ template <bool BF16> __device__ __forceinline__ RowParams ParamsOf(float hi, flo
         scale = mid = BF16 ? 0x7fc0u : 0x7e00u; // NaN
     }
     const float s = Widen<BF16>(scale);
-    p.inv = (bad || s == 0.0f) ? 0.0f : 1.0f / s;
+    p.inv = (bad || s == 0.0f) ? 0.0f : __builtin_amdgcn_rcpf(s); // (within an ulp: see Codes8)
     p.scale = s;
     p.mid = bad ? 0.0f : Widen<BF16>(mid);
     p.word = static_cast<uint32_t>(scale) | (static_cast<uint32_t>(mid) << 16);
@@ -58,8 +71,8 @@ template <bool BF16> __device__ __forceinline__ RowParams ParamsOf(float hi, flo
 
 // Codes of eight values, the first in the lowest four bits: rint((x - mid) / scale + 7.5) in 0 .. 15; 8 where the scale is
 // 0 or the row is not finite (x is then ignored). All three numbers have few bits, so whole quotients, which the half makes
-// ties, are common: the product with 1 / scale is corrected by its remainder, which makes them exact, and ties go to the
-// even code as the definition has it. A sum with 1.5 2^23 is rounded to a whole number, which its lowest bits then are.
+// ties, are common: the product with a reciprocal that is a little off is corrected by its remainder, which makes them exact,
+// and ties go to the even code as the definition has it. A sum with 1.5 2^23 is rounded to a whole number, which its lowest bits then are.
 __device__ __forceinline__ uint32_t Codes8(const float (&x)[8], const RowParams &p)
 {
     constexpr float MAGIC = 12582912.0f;

@@ -745,8 +745,8 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
                         const int cc = ct * HT + n;
                         uint16_t *dst = a.out + ((static_cast<int64_t>(seq) * a.tokens + cc / a.group) * a.H + g * a.group + cc % a.group) * D + d;
                         u32x2 w;
-                        w[0] = static_cast<uint32_t>(Narrow<BF16>(o[0] * inv)) | (static_cast<uint32_t>(Narrow<BF16>(o[1] * inv)) << 16);
-                        w[1] = static_cast<uint32_t>(Narrow<BF16>(o[2] * inv)) | (static_cast<uint32_t>(Narrow<BF16>(o[3] * inv)) << 16);
+                        w[0] = NarrowPair<BF16>(o[0] * inv, o[1] * inv);
+                        w[1] = NarrowPair<BF16>(o[2] * inv, o[3] * inv);
                         *reinterpret_cast<u32x2 *>(dst) = w;
                     } else {
                         *reinterpret_cast<f32x4 *>(a.partO + (part * HT + n) * D + d) = o;
@@ -857,8 +857,8 @@ template <int D, bool BF16> __global__ __launch_bounds__(MERGE_MOST_THREADS) voi
             const int cc = ct * HT + n;
             uint16_t *dst = a.out + ((static_cast<int64_t>(seq) * a.tokens + cc / a.group) * a.H + g * a.group + cc % a.group) * D + 4 * q;
             u32x2 w;
-            w[0] = static_cast<uint32_t>(Narrow<BF16>(o[0] * inv)) | (static_cast<uint32_t>(Narrow<BF16>(o[1] * inv)) << 16);
-            w[1] = static_cast<uint32_t>(Narrow<BF16>(o[2] * inv)) | (static_cast<uint32_t>(Narrow<BF16>(o[3] * inv)) << 16);
+            w[0] = NarrowPair<BF16>(o[0] * inv, o[1] * inv);
+            w[1] = NarrowPair<BF16>(o[2] * inv, o[3] * inv);
             *reinterpret_cast<u32x2 *>(dst) = w;
         }
     }

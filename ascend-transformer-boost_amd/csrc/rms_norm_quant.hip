@@ -12,6 +12,7 @@ namespace atbmi {
 namespace normq {
 
 using int4kv::Narrow;
+using int4kv::NarrowPair;
 using int4kv::Widen;
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
@@ -181,9 +182,9 @@ template <bool BF16, bool RES, int NV> __global__ __launch_bounds__(MOST_THREADS
         for (int v = 0; v < NV; ++v) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint16_t lo = Narrow<BF16>(Widen<BF16>(static_cast<uint16_t>(s[v][i])) + Widen<BF16>(static_cast<uint16_t>(add[v][i])));
-                const uint16_t hi = Narrow<BF16>(Widen<BF16>(static_cast<uint16_t>(s[v][i] >> 16)) + Widen<BF16>(static_cast<uint16_t>(add[v][i] >> 16)));
-                s[v][i] = lo | (static_cast<uint32_t>(hi) << 16);
+                s[v][i] = NarrowPair<BF16>(
+                    Widen<BF16>(static_cast<uint16_t>(s[v][i])) + Widen<BF16>(static_cast<uint16_t>(add[v][i])),
+                    Widen<BF16>(static_cast<uint16_t>(s[v][i] >> 16)) + Widen<BF16>(static_cast<uint16_t>(add[v][i] >> 16)));
             }
             const int at = static_cast<int>(threadIdx.x) + v * T;
             if (at < pieces && a.residualOut) {
