@@ -48,15 +48,11 @@ __device__ __forceinline__ s16x2 Ordered(uint32_t word)
     return Ordered(__builtin_bit_cast(s16x2, word));
 }
 
-struct RowCodes {
-    uint32_t codes; // of the lane's eight values
-    RowParams params;
-};
-
-// Quantises a row that LPR lanes hold, eight values each (w: as they are read). Maximum and minimum are taken on the 16-bit
-// values as integers, two to an instruction, the minimum as the maximum of the complements in the other half of a word:
-// the kernel for many tokens was bound by its arithmetic, 208 instructions for eight values, half of them for this.
-template <int LPR, bool BF16> __device__ __forceinline__ RowCodes CodesOf(const u32x4 w)
+// Largest and smallest value of a row that LPR lanes hold, eight values each (w: as they are read), as 16-bit floats in the
+// low and high half. Both are found on integers, two values to an instruction, the minimum as the maximum of the
+// complements in the other half of a word: the kernel for many tokens was bound by its arithmetic, 208 instructions for
+// eight values, half of them for this.
+template <int LPR> __device__ __forceinline__ uint32_t SpanOf(const u32x4 w)
 {
     s16x2 hi = Ordered(w[0]), lo = hi;
 #pragma unroll
@@ -77,19 +73,34 @@ template <int LPR, bool BF16> __device__ __forceinline__ RowCodes CodesOf(const 
         span = __builtin_elementwise_max(span, __builtin_bit_cast(s16x2, __shfl_xor(__builtin_bit_cast(int, span), 16)));
     }
     span[1] = ~span[1];
-    span = Ordered(span);
-    constexpr int INF = BF16 ? 0x7f80 : 0x7c00;
-    const bool bad = (span[0] & 0x7fff) >= INF || (span[1] & 0x7fff) >= INF; // an infinity or NaN somewhere in the row
+    return __builtin_bit_cast(uint32_t, Ordered(span));
+}
+
+template <bool BF16> __device__ __forceinline__ RowParams ParamsOfSpan(uint32_t span)
+{
+    constexpr uint32_t INF = BF16 ? 0x7f80u : 0x7c00u;
+    const bool bad = (span & 0x7fffu) >= INF || ((span >> 16) & 0x7fffu) >= INF; // an infinity or NaN somewhere in the row
+    return ParamsOf<BF16>(Widen<BF16>(static_cast<uint16_t>(span)), Widen<BF16>(static_cast<uint16_t>(span >> 16)), bad);
+}
+
+// The parameters that lane LANE of four neighbouring ones holds.
+template <int LANE> __device__ __forceinline__ void FromQuad(const RowParams &p, float &mid, float &inv, uint32_t &word)
+{
+    mid = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(p.mid), LANE * 0x55, 0xf, 0xf, true));
+    inv = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(p.inv), LANE * 0x55, 0xf, 0xf, true));
+    word = static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(p.word), LANE * 0x55, 0xf, 0xf, true));
+}
+
+// The lane's eight values against the row's parameters.
+template <bool BF16> __device__ __forceinline__ uint32_t CodesOf(const u32x4 w, float mid, float inv)
+{
     float x[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         x[2 * i] = Widen<BF16>(static_cast<uint16_t>(w[i]));
         x[2 * i + 1] = Widen<BF16>(static_cast<uint16_t>(w[i] >> 16));
     }
-    RowCodes r;
-    r.params = ParamsOf<BF16>(Widen<BF16>(static_cast<uint16_t>(span[0])), Widen<BF16>(static_cast<uint16_t>(span[1])), bad);
-    r.codes = Codes8(x, r.params);
-    return r;
+    return Codes8(x, mid, inv);
 }
 
 // One row (token, head) to D / 8 lanes; blockIdx.y: 0 keys, 1 values.
@@ -115,7 +126,8 @@ __global__ __launch_bounds__(MOVE_THREADS) void WriteKernel(const WriteArgs a)
             w[i] = src[2 * i] | (static_cast<uint32_t>(src[2 * i + 1]) << 16);
         }
     }
-    const RowCodes r = CodesOf<LPR, BF16>(w);
+    const RowParams params = ParamsOfSpan<BF16>(SpanOf<LPR>(w));
+    const uint32_t codes = CodesOf<BF16>(w, params.mid, params.inv);
     if (slot < 0 || slot >= a.numSlots) {
         return; // (after the last cross-lane step)
     }
@@ -126,20 +138,20 @@ __global__ __launch_bounds__(MOVE_THREADS) void WriteKernel(const WriteArgs a)
         uint8_t *dst = a.valueCache + (head * (D / 2) + l * 4) * a.blockSize + at;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            dst[static_cast<int64_t>(i) * a.blockSize] = static_cast<uint8_t>(r.codes >> (8 * i));
+            dst[static_cast<int64_t>(i) * a.blockSize] = static_cast<uint8_t>(codes >> (8 * i));
         }
     } else {
-        *reinterpret_cast<uint32_t *>(a.keyCache + (head * a.blockSize + at) * (D / 2) + l * 4) = r.codes;
+        *reinterpret_cast<uint32_t *>(a.keyCache + (head * a.blockSize + at) * (D / 2) + l * 4) = codes;
     }
     if (l == 0) {
-        (isValue ? a.valueParams : a.keyParams)[head * a.blockSize + at] = r.params.word;
+        (isValue ? a.valueParams : a.keyParams)[head * a.blockSize + at] = params.word;
     }
 }
 
 // The same for many tokens: a workgroup takes 64 tokens of one head, a wave 16 of them. Value codes lie token after token in
 // the cache, so they are turned in LDS: a wave then stores 64 neighbouring tokens' bytes of one channel pair at a time,
 // which the memory takes as one piece where the tokens' slots follow each other (as a prompt's do) and byte by byte where
-// they do not. (2048 new tokens of 5 sequences with 8 heads of 128 channels: 40 -> 21 us, against bytes stored from
+// they do not. (2048 new tokens of 5 sequences with 8 heads of 128 channels: 40 -> 17 us, against bytes stored from
 // the lanes of the row; one token a call of 512 sequences: 7 us in rows, 11 us in tiles, so that fewer than 1024 go in rows.)
 constexpr int TILE_TOKENS = 64;
 constexpr int TILE_FROM = 1024;
@@ -175,26 +187,46 @@ __global__ __launch_bounds__(MOVE_THREADS) void WriteTileKernel(const WriteArgs 
             }
         }
     }
+    // The parameters of four rows at a time: each of four neighbouring lanes works out those of one, and gives them to the
+    // other three.
+    float mid[STEPS], inv[STEPS];
+    uint32_t word[STEPS];
+#pragma unroll
+    for (int s0 = 0; s0 < STEPS; s0 += 4) {
+        uint32_t span = SpanOf<LPR>(w[s0]);
+#pragma unroll
+        for (int s = 1; s < 4 && s0 + s < STEPS; ++s) {
+            const uint32_t other = SpanOf<LPR>(w[s0 + s]);
+            span = lane % 4 == s ? other : span;
+        }
+        const RowParams p = ParamsOfSpan<BF16>(span);
+        FromQuad<0>(p, mid[s0], inv[s0], word[s0]);
+        FromQuad<1>(p, mid[s0 + 1], inv[s0 + 1], word[s0 + 1]);
+        if constexpr (STEPS > 2) {
+            FromQuad<2>(p, mid[s0 + 2], inv[s0 + 2], word[s0 + 2]);
+            FromQuad<3>(p, mid[s0 + 3], inv[s0 + 3], word[s0 + 3]);
+        }
+    }
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
         const int t = wave * 16 + s * ROWS + lane / LPR; // (past the last token: the last one again, not stored)
-        const RowCodes row = CodesOf<LPR, BF16>(w[s]);
+        const uint32_t codes = CodesOf<BF16>(w[s], mid[s], inv[s]);
         if (isValue) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                turned[4 * l + i][t] = static_cast<uint8_t>(row.codes >> (8 * i));
+                turned[4 * l + i][t] = static_cast<uint8_t>(codes >> (8 * i));
             }
             if (l == 0) {
-                params[t] = row.params.word;
+                params[t] = word[s];
             }
         } else if (t < tokens) {
             const int64_t slot = a.slots[token0 + t];
             if (slot >= 0 && slot < a.numSlots) {
-                const int64_t block = static_cast<int32_t>(slot) / a.blockSize;
-                const int64_t at = (block * a.G + g) * a.blockSize + (slot - block * a.blockSize);
-                *reinterpret_cast<uint32_t *>(a.keyCache + at * (D / 2) + l * 4) = row.codes;
+                const int32_t block = static_cast<int32_t>(slot) / a.blockSize;
+                const int64_t at = (static_cast<int64_t>(block) * a.G + g) * a.blockSize + (static_cast<int32_t>(slot) - block * a.blockSize);
+                *reinterpret_cast<uint32_t *>(a.keyCache + at * (D / 2) + l * 4) = codes;
                 if (l == 0) {
-                    a.keyParams[at] = row.params.word;
+                    a.keyParams[at] = word[s];
                 }
             }
         }
@@ -268,7 +300,9 @@ template <bool BF16> __device__ __forceinline__ u32x4 Expand(uint32_t codes, flo
 // group that holds the sequence's first one: lane (l, grp) owns channels 8 l .. 8 l + 7 of the 16 positions of its group,
 // which lie in one block. Everything is asked for before the first row is stored. Value codes lie token after token, so the
 // lane reads four 16-byte runs (its four channel pairs) and turns them by 4 x 4 byte transpositions; no shared memory. One
-// wave a workgroup: a short prefix is spread over as many CUs as it has pieces.
+// wave a workgroup: a short prefix is spread over as many CUs as it has pieces. Tables reach further than most sequences
+// go, but a workgroup that finds nothing is cheap: with fewer, each going on with later pieces, the longest sequences came
+// last (16 sequences with 65000 rows 79 us, 90 with at most 32 workgroups a CU).
 template <int D, bool BF16>
 __global__ __launch_bounds__(WAVE) void LoadKernel(const LoadArgs a)
 {

@@ -40,7 +40,6 @@ template <bool BF16> __device__ __forceinline__ float MidOf(uint32_t word)
 
 struct RowParams {
     float inv; // 1 / scale, 0 where the scale is 0
-    float scale;
     float mid;
     uint32_t word;
 };
@@ -63,7 +62,6 @@ template <bool BF16> __device__ __forceinline__ RowParams ParamsOf(float hi, flo
     }
     const float s = Widen<BF16>(scale);
     p.inv = (bad || s == 0.0f) ? 0.0f : __builtin_amdgcn_rcpf(s); // (within an ulp: see Codes8)
-    p.scale = s;
     p.mid = bad ? 0.0f : Widen<BF16>(mid);
     p.word = static_cast<uint32_t>(scale) | (static_cast<uint32_t>(mid) << 16);
     return p;
@@ -71,22 +69,22 @@ template <bool BF16> __device__ __forceinline__ RowParams ParamsOf(float hi, flo
 
 // Codes of eight values, the first in the lowest four bits: rint((x - mid) / scale + 7.5) in 0 .. 15; 8 where the scale is
 // 0 or the row is not finite (x is then ignored). All three numbers have few bits, so whole quotients, which the half makes
-// ties, are common: the product with a reciprocal that is a little off is corrected by its remainder, which makes them exact,
-// and ties go to the even code as the definition has it. A sum with 1.5 2^23 is rounded to a whole number, which its lowest bits then are.
-__device__ __forceinline__ uint32_t Codes8(const float (&x)[8], const RowParams &p)
+// ties, are common, and ties go to the even code. Sums with 96 are rounded to 2^-17 and sums with 1.5 2^23 to whole numbers,
+// which the lowest bits then are: the first makes a tie of every quotient that is one (the product with a reciprocal that
+// is a little off is within 2^-19 of it), at the price that places within 2^-18 of the middle between two codes count as
+// ties as well; the second rounds to the even code.
+__device__ __forceinline__ uint32_t Codes8(const float (&x)[8], float mid, float inv)
 {
-    constexpr float MAGIC = 12582912.0f;
+    constexpr float SNAP = 96.0f, MAGIC = 12582912.0f;
     uint32_t codes = 0, extra = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float d = x[i] - p.mid;
-        const float q0 = d * p.inv;
-        const float quotient = __builtin_fmaf(__builtin_fmaf(-q0, p.scale, d), p.inv, q0);
-        const float q = __builtin_amdgcn_fmed3f(quotient + 7.5f, 0.0f, 15.0f) + MAGIC;
+        const float place = __builtin_fmaf(x[i] - mid, inv, SNAP + 7.5f);
+        const float q = __builtin_amdgcn_fmed3f(place, SNAP, SNAP + 15.0f) + (MAGIC - SNAP);
         codes += __float_as_uint(q) << (4 * i);
         extra += 0x4b400000u << (4 * i); // the bits of MAGIC
     }
-    return p.inv == 0.0f ? 0x88888888u : codes - extra;
+    return inv == 0.0f ? 0x88888888u : codes - extra;
 }
 
 inline int CheckCache(const char *who, int32_t dtype, int64_t numKvHeads, int64_t headDim, int64_t blockSize,
