@@ -165,6 +165,7 @@ def test_outputs_of_another_shape_or_place(binding):
 def test_execute_wants_the_workspace(binding):
     """A long context is worked on by several workgroups, whose parts need room."""
     name, param, ins, outs, alias = _attend(binding)
+    ins[5] = ("int32", [3, 400])
     op = binding.Operation(name, param)
     context = binding.Context(0x77)
     tensors, outputs = _tensors(binding, ins), _tensors(binding, outs)
