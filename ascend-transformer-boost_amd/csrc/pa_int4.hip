@@ -22,7 +22,7 @@
 //   values   O^T = V^T P^T: A = value codes, which lie token after token (16 tokens of a channel pair are 16 bytes: a
 //            lane's tokens 16 kg .. + 15), B = the lane's own 16 weights. With 16 columns the weights stay in the lane
 //            that has the scores; with fewer, scores and weights pass through LDS once so that no lane computes the
-//            softmax of a repeated column (batch of 64, 4 columns, 1024 to 4096 tokens: 54.4 -> 50.2 us).
+//            softmax of a repeated column (batch of 64, 4 columns, 1024 to 4096 tokens: 54 -> 50 us).
 // Running maximum and sums are fp32. The maximum a column is scaled by moves only when a score exceeds it by more
 // than 2^8 (in the exponent: 8): weights up to 256 are as exact as weights up to 1, and the accumulators are rescaled
 // a few times a context instead of every tile.
@@ -185,7 +185,9 @@ __device__ __forceinline__ uint32_t PackBf16(float a, float b)
 }
 
 // 16 bytes (4 bytes) a lane to LDS at ldsAt + 16 (4) x lane, from an address of its own or from an offset to the wave's;
-// read once, so not to displace anything.
+// read once, so not to displace anything. Value codes in long blocks are left in the L2 a while (Kept): a 64-token tile takes
+// half of each 128-byte line of theirs, and the wave that takes the other half comes about the same time (fp16, batch of 128 with
+// 2048 .. 8192 tokens: 172 -> 165 us, keys without the hint as well: 185 us; with 64 and 256 channels 3 % slower).
 __device__ __forceinline__ void ToLds16(const void *from, uint32_t ldsAt)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(ldsAt), "v"(from) : "memory", "m0");
@@ -201,6 +203,10 @@ __device__ __forceinline__ void ToLds16(const void *base, uint32_t offset, uint3
 __device__ __forceinline__ void ToLds4(const void *base, uint32_t offset, uint32_t ldsAt)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2 nt" ::"s"(ldsAt), "v"(offset), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void ToLds16Kept(const void *base, uint32_t offset, uint32_t ldsAt)
+{
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(ldsAt), "v"(offset), "s"(base) : "memory", "m0");
 }
 // Orders a wave's LDS writes before its own later reads and the other way round: a wave's LDS instructions execute in
 // order, only the compiler has to keep them.
@@ -262,8 +268,8 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
     const int pairs = a.G * a.colTiles;
     const int range = blockIdx.x / pairs;
     const int pair = blockIdx.x % pairs;
-    const int g = pair / a.colTiles;
-    const int ct = pair % a.colTiles;
+    const int g = pair % a.G; // (the column tiles of a head are G workgroups apart: with 8 heads on the same XCD and its L2)
+    const int ct = pair / a.G;
 
     // ---- where the range begins
     int begin = 0, end = 1; // (of a whole sequence: any, it ends after the first)
@@ -349,7 +355,11 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
                 }
 #pragma unroll
                 for (int i = 0; i < CT; ++i) {
-                    ToLds16(v + i * 16 * a.blockSize, valueAt, to + L::KEYS + i * 1024);
+                    if constexpr (D == 128) {
+                        ToLds16Kept(v + i * 16 * a.blockSize, valueAt, to + L::KEYS + i * 1024);
+                    } else {
+                        ToLds16(v + i * 16 * a.blockSize, valueAt, to + L::KEYS + i * 1024);
+                    }
                 }
                 const int64_t param = head * a.blockSize + place;
                 ToLds4(a.kp + param, 4 * lane, to + L::PARAMS);
@@ -788,8 +798,8 @@ template <int D, bool BF16> __global__ __launch_bounds__(MERGE_MOST_THREADS) voi
     const int pairs = a.G * a.colTiles;
     const int seq = blockIdx.x / pairs;
     const int pair = blockIdx.x % pairs;
-    const int g = pair / a.colTiles;
-    const int ct = pair % a.colTiles;
+    const int g = pair % a.G;
+    const int ct = pair / a.G;
     int units = 0, before = 0;
     for (int b = lane; b < a.batch; b += WAVE) {
         const int own = UnitsOf(ContextLen(a, b));
