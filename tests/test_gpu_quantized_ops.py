@@ -171,3 +171,19 @@ def test_write_of_many_tokens(ops, dev, tokens, heads, d, block, gap, order, dty
         before[i][s // block, :, s % block] = after[i][s // block, :, s % block]
     before[1][s // block, :, :, s % block] = after[1][s // block, :, :, s % block]
     assert all(_same(a, b) for a, b in zip(before, after))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("rows,dim", [(515, 4096), (513, 8192), (512, 8200), (600, 1032), (530, 16384), (512, 40000), (700, 777)])
+def test_norm_of_many_rows(ops, dev, rows, dim, dtype):
+    """Rows enough to fill the chip, where a row gets fewer threads; with special rows among them."""
+    gen = _gen(rows + dim)
+    x = torch.randn(rows, dim, generator=gen).to(dtype)
+    r = torch.randn(rows, dim, generator=gen).to(dtype)
+    x[3], r[3] = 0, 0
+    x[5] = (x[5].float() * 1e-3).to(dtype)
+    gamma = torch.randn(dim, generator=gen).to(dtype)
+    for residual in (None, r):
+        codes, scale, out = ops.rms_norm_quant(x.to(dev), gamma.to(dev), residual=None if residual is None else residual.to(dev))
+        assert qo.norm_quant_ok(x, residual, gamma, 1e-5, codes.cpu(), scale.cpu(), out.cpu())
+        assert float(scale[3]) == 0 and bool((codes[3] == 0).all())
