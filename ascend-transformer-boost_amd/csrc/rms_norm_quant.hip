@@ -176,20 +176,20 @@ template <bool BF16, bool RES, int NV> __global__ __launch_bounds__(MOST_THREADS
             held[v] = gamma[min(static_cast<int>(threadIdx.x) + v * T, pieces - 1)];
         }
     }
-    if constexpr (RES) {
-        u32x4 *ro = reinterpret_cast<u32x4 *>(a.residualOut + row * a.dim);
+    u32x4 *ro = reinterpret_cast<u32x4 *>(a.residualOut + row * a.dim);
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
+    for (int v = 0; v < NV; ++v) {
+        if constexpr (RES) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 s[v][i] = NarrowPair<BF16>(
                     Widen<BF16>(static_cast<uint16_t>(s[v][i])) + Widen<BF16>(static_cast<uint16_t>(add[v][i])),
                     Widen<BF16>(static_cast<uint16_t>(s[v][i] >> 16)) + Widen<BF16>(static_cast<uint16_t>(add[v][i] >> 16)));
             }
-            const int at = static_cast<int>(threadIdx.x) + v * T;
-            if (at < pieces && a.residualOut) {
-                ro[at] = s[v];
-            }
+        }
+        const int at = static_cast<int>(threadIdx.x) + v * T;
+        if (at < pieces && a.residualOut) {
+            ro[at] = s[v];
         }
     }
     auto pass = [&](float pre, float &sumSq, float &maxSg, float &maxS) __attribute__((always_inline)) {

@@ -1,0 +1,51 @@
+"""The quantised decoder-layer operators at the edges of what their definition allows, against 64-bit plain implementations:
+outputs that only the C ABI offers, values at the ends of the types' ranges, launches of many rows."""
+import pytest
+import torch
+
+import quant_oracle as qo
+from test_gpu_quantized import DTYPES, _gen, _randn
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops(pkg):
+    return pkg.quantized
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "these tests need the MI355X"
+    return torch.device("cuda:0")
+
+
+def _norm_c(binding, dev, x, gamma, eps, residual_out, out, scale):
+    """atbmi_rms_norm_quant without a residual."""
+    code = binding.ATBMI_F16 if x.dtype == torch.float16 else binding.ATBMI_BF16
+    rc = binding.kernels().atbmi_rms_norm_quant(x.data_ptr(), None, gamma.data_ptr(), out.data_ptr(), scale.data_ptr(),
+                                                residual_out.data_ptr(), x.shape[0], x.shape[1], x.stride(0), 0, code, eps,
+                                                torch.cuda.current_stream(dev).cuda_stream)
+    assert rc == 0, binding.kernels().atbmi_last_error()
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("gap", [0, 8])
+@pytest.mark.parametrize("rows,dim", [(3, 64), (600, 2048), (7, 4096), (7, 4099), (600, 8192), (2, 65536)])
+def test_norm_quant_gives_its_rows_without_a_residual(binding, dev, rows, dim, gap, dtype):
+    """residualOut holds x where there is no residual, whatever the rows' length and stride; so it does where it is x."""
+    gen = _gen(rows + dim)
+    x, gamma = _randn(gen, (rows, dim + gap), dtype), _randn(gen, (dim,), dtype)
+    dx, dgamma = x.to(dev), gamma.to(dev)
+    out = torch.full((rows, dim), 99, dtype=torch.int8, device=dev)
+    scale = torch.full((rows,), -1.0, device=dev)
+    kept = torch.full((rows + 1, dim), -7.0, dtype=dtype, device=dev)
+    _norm_c(binding, dev, dx[:, :dim], dgamma, 1e-5, kept, out, scale)
+    assert torch.equal(kept[:rows].cpu(), x[:, :dim]) and bool((kept[rows] == -7.0).all())
+    assert torch.equal(dx.cpu(), x)
+    assert qo.norm_quant_ok(x[:, :dim], None, gamma, 1e-5, out.cpu(), scale.cpu(), None)
+    if gap == 0:
+        again, again_scale = torch.empty_like(out), torch.empty_like(scale)
+        _norm_c(binding, dev, dx, dgamma, 1e-5, dx, again, again_scale)
+        assert torch.equal(dx.cpu(), x) and torch.equal(again, out) and torch.equal(again_scale, scale)
