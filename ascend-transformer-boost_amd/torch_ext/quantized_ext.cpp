@@ -108,14 +108,21 @@ Tensor Empty(at::IntArrayRef sizes, ScalarType type, c10::Device device)
     return at::empty(sizes, c10::TensorOptions().dtype(type).device(device));
 }
 
+// Address of a tensor's first value, null for no tensor. It raises for a tensor without memory of its own (torch.vmap's, a
+// FakeTensor), so it is asked for in front of Unlocked and of anything that is done on the device.
+template <typename T = void> T *At(const Tensor *t)
+{
+    return t != nullptr ? static_cast<T *>(t->data_ptr()) : nullptr;
+}
+
 // The C ABI is called without the interpreter's lock: a launch may wait for room in the device's queue.
 template <typename F> int Unlocked(F call)
 {
-    int rc;
-    Py_BEGIN_ALLOW_THREADS
-    rc = call();
-    Py_END_ALLOW_THREADS
-    return rc;
+    struct Released {
+        PyThreadState *const state = PyEval_SaveThread();
+        ~Released() { PyEval_RestoreThread(state); } // (by an exception's way out as well)
+    } const released;
+    return call();
 }
 
 PyObject *Failed(int rc)
@@ -166,15 +173,17 @@ PyObject *RmsNormQuant(PyObject *, PyObject *const *items, Py_ssize_t count)
         (a.Given(6) && !IsWhole(a.Get(6), type, x->sizes(), device))) {
         Py_RETURN_NONE;
     }
+    const void *xAt = At(x), *rAt = At(residual), *gammaAt = At(gamma);
     const c10::DeviceGuard guard(device);
     Tensor out = a.Given(4) ? *a.Get(4) : Empty({rows, dim}, ScalarType::Char, device);
     Tensor scale = a.Given(5) ? *a.Get(5) : Empty({rows}, ScalarType::Float, device);
     Tensor sum = a.Given(6) ? *a.Get(6) : (residual ? Empty({rows, dim}, type, device) : *x);
+    int8_t *outAt = At<int8_t>(&out);
+    float *scaleAt = At<float>(&scale);
+    void *sumAt = residual ? At(&sum) : nullptr;
     void *stream = Stream(device);
     const int rc = rows == 0 ? 0 : Unlocked([&] {
-        return atbmi_rms_norm_quant(x->data_ptr(), residual ? residual->data_ptr() : nullptr, gamma->data_ptr(),
-                                    static_cast<int8_t *>(out.data_ptr()), static_cast<float *>(scale.data_ptr()),
-                                    residual ? sum.data_ptr() : nullptr, rows, dim, xStride, rStride, Code(type), epsilon,
+        return atbmi_rms_norm_quant(xAt, rAt, gammaAt, outAt, scaleAt, sumAt, rows, dim, xStride, rStride, Code(type), epsilon,
                                     stream);
     });
     if (rc != 0) {
@@ -226,6 +235,8 @@ PyObject *LinearInt8(PyObject *, PyObject *const *items, Py_ssize_t count)
     if (!IsModelType(type) || (given && (!Is(given, type, {m, n}, device) || RowStride(*given) < 0))) {
         Py_RETURN_NONE;
     }
+    const int8_t *xAt = At<int8_t>(x), *wAt = At<int8_t>(w);
+    const float *xScaleAt = At<float>(xScale), *wScaleAt = At<float>(wScale), *biasAt = At<float>(bias);
     const c10::DeviceGuard guard(device);
     Tensor out = given ? *given : Empty({m, n}, type, device);
     if (m != 0 && n != 0) {
@@ -238,14 +249,12 @@ PyObject *LinearInt8(PyObject *, PyObject *const *items, Py_ssize_t count)
         if (need > 0) {
             workspace = Empty({static_cast<int64_t>(need)}, ScalarType::Byte, device);
         }
-        void *at = need > 0 ? workspace.data_ptr() : nullptr;
+        void *outAt = At(&out), *at = need > 0 ? At(&workspace) : nullptr;
+        const int64_t outStride = RowStride(out);
         void *stream = Stream(device);
         rc = Unlocked([&] {
-            return atbmi_linear_int8(static_cast<const int8_t *>(x->data_ptr()), static_cast<const int8_t *>(w->data_ptr()),
-                                     static_cast<const float *>(xScale->data_ptr()),
-                                     static_cast<const float *>(wScale->data_ptr()),
-                                     bias ? static_cast<const float *>(bias->data_ptr()) : nullptr, out.data_ptr(), m, n, k,
-                                     xStride, wStride, RowStride(out), Code(type), at, need, stream);
+            return atbmi_linear_int8(xAt, wAt, xScaleAt, wScaleAt, biasAt, outAt, m, n, k, xStride, wStride, outStride, Code(type),
+                                     at, need, stream);
         });
         if (rc != 0) {
             return Failed(rc);
@@ -265,6 +274,8 @@ struct Cache {
     ScalarType type = ScalarType::Undefined;
     c10::Device device{c10::kCPU};
     int64_t blocks = 0, heads = 0, block = 0, half = 0;
+    uint8_t *keys = nullptr, *values = nullptr; // where they lie: see At
+    void *keyParams = nullptr, *valueParams = nullptr;
 
     bool Read(Args &a, int at)
     {
@@ -278,6 +289,10 @@ struct Cache {
         return IsWhole(kc, ScalarType::Byte, kc->sizes(), device) &&
                IsWhole(vc, ScalarType::Byte, {blocks, heads, half, block}, device) &&
                IsWhole(kp, type, {blocks, heads, block, 2}, device) && IsWhole(vp, type, {blocks, heads, block, 2}, device);
+    }
+    void Locate()
+    {
+        keys = At<uint8_t>(kc), values = At<uint8_t>(vc), keyParams = At(kp), valueParams = At(vp);
     }
 };
 
@@ -300,14 +315,15 @@ PyObject *ReshapeAndCacheInt4(PyObject *, PyObject *const *items, Py_ssize_t cou
         Py_RETURN_NONE;
     }
     if (tokens != 0) {
+        c.Locate();
+        const void *keyAt = At(key), *valueAt = At(value);
+        const int32_t *slotsAt = At<int32_t>(slots);
+        const int64_t keyStride = TokenStride(*key), valueStride = TokenStride(*value);
         const c10::DeviceGuard guard(c.device);
         void *stream = Stream(c.device);
         const int rc = Unlocked([&] {
-            return atbmi_reshape_and_cache_int4(
-                key->data_ptr(), value->data_ptr(), static_cast<uint8_t *>(c.kc->data_ptr()),
-                static_cast<uint8_t *>(c.vc->data_ptr()), c.kp->data_ptr(), c.vp->data_ptr(),
-                static_cast<const int32_t *>(slots->data_ptr()), tokens, c.heads, d, c.block, c.blocks, TokenStride(*key),
-                TokenStride(*value), Code(c.type), stream);
+            return atbmi_reshape_and_cache_int4(keyAt, valueAt, c.keys, c.values, c.keyParams, c.valueParams, slotsAt, tokens,
+                                                c.heads, d, c.block, c.blocks, keyStride, valueStride, Code(c.type), stream);
         });
         if (rc != 0) {
             return Failed(rc);
@@ -340,18 +356,18 @@ PyObject *PagedCacheLoadInt4(PyObject *, PyObject *const *items, Py_ssize_t coun
         (a.Given(10) && !IsWhole(a.Get(10), c.type, {rows, c.heads, d}, c.device))) {
         Py_RETURN_NONE;
     }
+    c.Locate();
+    const int32_t *tablesAt = At<int32_t>(tables), *lensAt = At<int32_t>(lens), *startsAt = At<int32_t>(starts);
     const c10::DeviceGuard guard(c.device);
     Tensor key = a.Given(9) ? *a.Get(9) : Empty({rows, c.heads, d}, c.type, c.device);
     Tensor value = a.Given(10) ? *a.Get(10) : Empty({rows, c.heads, d}, c.type, c.device);
     if (batch != 0 && reach != 0 && rows != 0) {
+        void *keyAt = At(&key), *valueAt = At(&value);
         void *stream = Stream(c.device);
         const int rc = Unlocked([&] {
-            return atbmi_paged_cache_load_int4(
-                static_cast<const uint8_t *>(c.kc->data_ptr()), static_cast<const uint8_t *>(c.vc->data_ptr()),
-                c.kp->data_ptr(), c.vp->data_ptr(), static_cast<const int32_t *>(tables->data_ptr()),
-                static_cast<const int32_t *>(lens->data_ptr()),
-                starts ? static_cast<const int32_t *>(starts->data_ptr()) : nullptr, key.data_ptr(), value.data_ptr(), batch,
-                reach, c.heads, d, c.block, c.blocks, rows, longest, Code(c.type), stream);
+            return atbmi_paged_cache_load_int4(c.keys, c.values, c.keyParams, c.valueParams, tablesAt, lensAt, startsAt, keyAt,
+                                               valueAt, batch, reach, c.heads, d, c.block, c.blocks, rows, longest, Code(c.type),
+                                               stream);
         });
         if (rc != 0) {
             return Failed(rc);
@@ -409,9 +425,17 @@ PyObject *PagedAttentionInt4(PyObject *, PyObject *const *items, Py_ssize_t coun
             }
             *strides[i] = mask->size(i) > 1 ? mask->stride(i) : 0;
         }
-        call.mask = mask->data_ptr();
+        call.mask = At(mask);
         call.maskLen = static_cast<int32_t>(mask->size(3));
     }
+    c.Locate();
+    call.query = At(query);
+    call.keyCache = c.keys;
+    call.valueCache = c.values;
+    call.keyParams = c.keyParams;
+    call.valueParams = c.valueParams;
+    call.blockTables = At<int32_t>(tables);
+    call.contextLens = At<int32_t>(lens);
     const c10::DeviceGuard guard(c.device);
     Tensor out = a.Given(10) ? *a.Get(10) : Empty(query->sizes(), c.type, c.device);
     if (batch != 0) {
@@ -425,14 +449,7 @@ PyObject *PagedAttentionInt4(PyObject *, PyObject *const *items, Py_ssize_t coun
         call.batch = static_cast<int32_t>(batch);
         call.queryTokens = static_cast<int32_t>(tokens);
         call.qkScale = scale;
-        call.query = query->data_ptr();
-        call.keyCache = static_cast<const uint8_t *>(c.kc->data_ptr());
-        call.valueCache = static_cast<const uint8_t *>(c.vc->data_ptr());
-        call.keyParams = c.kp->data_ptr();
-        call.valueParams = c.vp->data_ptr();
-        call.blockTables = static_cast<const int32_t *>(tables->data_ptr());
-        call.contextLens = static_cast<const int32_t *>(lens->data_ptr());
-        call.out = out.data_ptr();
+        call.out = At(&out);
         uint64_t need = 0;
         int rc = atbmi_pa_int4_workspace_size(&call, &need);
         if (rc != 0) {
@@ -445,7 +462,7 @@ PyObject *PagedAttentionInt4(PyObject *, PyObject *const *items, Py_ssize_t coun
             workspace = Empty({static_cast<int64_t>(need)}, ScalarType::Byte, c.device);
         }
         const uint64_t size = workspace.defined() ? static_cast<uint64_t>(workspace.numel()) : 0;
-        void *at = size > 0 ? workspace.data_ptr() : nullptr;
+        void *at = size > 0 ? At(&workspace) : nullptr;
         void *stream = Stream(c.device);
         rc = Unlocked([&] { return atbmi_pa_int4_decode(&call, at, size, stream); });
         if (rc != 0) {

@@ -49,3 +49,15 @@ def test_norm_quant_gives_its_rows_without_a_residual(binding, dev, rows, dim, g
         again, again_scale = torch.empty_like(out), torch.empty_like(scale)
         _norm_c(binding, dev, dx, dgamma, 1e-5, dx, again, again_scale)
         assert torch.equal(dx.cpu(), x) and torch.equal(again, out) and torch.equal(again_scale, scale)
+
+
+def test_functions_under_vmap_raise(ops, dev):
+    """torch.vmap's tensors have no memory of their own: the call raises, and the next one runs as ever."""
+    x, gamma = torch.ones(3, 5, 96, dtype=torch.bfloat16, device=dev), torch.ones(96, dtype=torch.bfloat16, device=dev)
+    with pytest.raises(RuntimeError, match="data pointer"):
+        torch.vmap(lambda t: ops.rms_norm_quant(t, gamma)[1])(x)
+    x8, w = torch.ones(3, 5, 96, dtype=torch.int8, device=dev), torch.ones(8, 96, dtype=torch.int8, device=dev)
+    one = torch.ones(8, device=dev)
+    with pytest.raises(RuntimeError, match="data pointer"):
+        torch.vmap(lambda t: ops.linear_int8(t, w, one[:5], one, out_dtype=torch.bfloat16))(x8)
+    assert bool((ops.linear_int8(x8[0], w, one[:5], one, out_dtype=torch.bfloat16) == 96.0).all())
