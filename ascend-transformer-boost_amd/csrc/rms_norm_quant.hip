@@ -66,21 +66,26 @@ struct RowFactors {
     bool bad;
 };
 
-// Power of two that a row is multiplied by before its squares and products are taken: 1 but for rows of finite values
-// that leave fp32's range on the way (bf16 values past 1e19, whose squares are infinite, or below 2^-50, whose squares
-// lose bits or vanish). Such a row is taken a second time. (The factor for small rows keeps eps pre^2 finite.)
+constexpr float LEAST = 0x1p-118f; // (127 / LEAST is finite)
+
+// Power of two that a row is multiplied by before its squares and products are taken: 1 but for rows of finite values that
+// leave fp32's range on the way: bf16 values past 1e19, whose squares are infinite, or below 2^-50, whose squares lose bits
+// or vanish, and products with gamma past either end. Such a row is taken a second time, its largest value brought between
+// a half and one. With a large eps it is brought up only as far as eps pre^2 stays finite: its squares are then lost in
+// eps, where they would be lost in any case.
 __device__ __forceinline__ float PreOf(float sumSq, float maxSg, float maxS, float eps)
 {
     if (!__builtin_isfinite(maxS) || maxS == 0.0f || sumSq != sumSq) {
         return 1.0f;
     }
-    if (__builtin_isinf(sumSq) || __builtin_isinf(maxSg)) {
-        return __builtin_ldexpf(1.0f, -min(__builtin_amdgcn_frexp_expf(maxS), 126));
+    if (__builtin_isfinite(sumSq) && __builtin_isfinite(maxSg) && maxS >= 0x1p-50f && maxSg >= LEAST && eps < 0x1p126f) {
+        return 1.0f;
     }
-    if (maxS < 0x1p-50f) {
-        return eps > 0.0f ? 0x1p63f : 0x1p126f;
+    int power = min(-__builtin_amdgcn_frexp_expf(maxS), 126);
+    if (eps > 0.0f) {
+        power = min(power, (126 - __builtin_amdgcn_frexp_expf(eps)) >> 1);
     }
-    return 1.0f;
+    return __builtin_ldexpf(1.0f, power);
 }
 
 // From the sum of squares and max|s gamma| of a row multiplied by `pre`.
@@ -90,7 +95,7 @@ __device__ __forceinline__ RowFactors FactorsOf(float sumSq, float maxSg, int di
     f.pre = pre;
     f.bad = !__builtin_isfinite(sumSq) || !__builtin_isfinite(maxSg);
     const float rstd = rsqrtf(sumSq / static_cast<float>(dim) + eps * pre * pre);
-    const bool none = !(maxSg >= 0x1p-118f); // (127 / maxSg stays finite)
+    const bool none = !(maxSg >= LEAST);
     f.scale = f.bad ? __builtin_nanf("") : (none ? 0.0f : maxSg * rstd * (1.0f / 127.0f));
     f.step = (f.bad || none) ? 0.0f : 127.0f / maxSg;
     return f;

@@ -659,9 +659,10 @@ int atbmi_mla_mask_free_expand(const AtbmiMlaMaskFreeCall *call, void *workspace
  *   s = x[i] + residual[i] rounded to dtype (residual NULL: s = x[i]), stored to residualOut[i] unless that is NULL
  *   y = s * gamma / sqrt(mean(s^2) + epsilon)          (fp32, not rounded in between)
  *   scale[i] = max|y| / 127,  out[i] = rint(y / scale[i]) in [-127, 127]     (ties to even; max|y| = 0: scale 0, codes 0)
- * A row with a value (or gamma with one) that is not finite gets scale NaN and codes 0; one whose products s * gamma all
- * lie below 2^-118 counts as zeros. x and residual have row strides of their own
- * (elements, >= dim); out and residualOut are [rows, dim] without gaps. residualOut may be x or residual itself
+ * A row with a value (or gamma with one) that is not finite gets scale NaN and codes 0. Rows of finite values may lie anywhere
+ * in dtype's range, and epsilon anywhere in fp32's; only a row whose products s * gamma all lie below 2^-118, also with s
+ * multiplied by the power of two that brings its largest value between a half and one, counts as zeros. x and residual have
+ * row strides of their own (elements, >= dim); out and residualOut are [rows, dim] without gaps. residualOut may be x or residual itself
  * when that has no gaps either. dtype (fp16 or bf16) is the type of x, residual, gamma and residualOut; dim <= 65536.
  */
 int atbmi_rms_norm_quant(const void *xDevice, const void *residualDevice, const void *gammaDevice, int8_t *outDevice,

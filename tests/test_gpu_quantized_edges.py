@@ -61,3 +61,28 @@ def test_functions_under_vmap_raise(ops, dev):
     with pytest.raises(RuntimeError, match="data pointer"):
         torch.vmap(lambda t: ops.linear_int8(t, w, one[:5], one, out_dtype=torch.bfloat16))(x8)
     assert bool((ops.linear_int8(x8[0], w, one[:5], one, out_dtype=torch.bfloat16) == 96.0).all())
+
+
+@pytest.mark.parametrize("dim", [256, 259])
+@pytest.mark.parametrize("epsilon", [0.0, 1e-30, 1e-5, 4.0, 1e30, 3.4e38])
+@pytest.mark.parametrize("gamma_power", [0, -110, 100, 127])
+def test_norm_quant_rows_anywhere_in_the_range(ops, dev, gamma_power, epsilon, dim):
+    """A row for every power of two of the bf16 range, and epsilons whose sum with the squares leaves fp32's unless both are
+    brought down: codes and scales as for any other row, wherever the scale is an fp32 number."""
+    gen = _gen(dim + gamma_power)
+    powers = torch.arange(-133, 128, dtype=torch.float64)
+    rows = (torch.rand((len(powers), dim), generator=gen, dtype=torch.float64) * 2 - 1)
+    rows[:, 0] = 1.0
+    x = (rows * torch.exp2(powers)[:, None]).to(torch.bfloat16)
+    gamma = ((torch.rand((dim,), generator=gen, dtype=torch.float64) + 0.9) * 2.0 ** gamma_power / 2).to(torch.bfloat16)
+    assert bool(x.isfinite().all()) and bool(gamma.isfinite().all())
+    codes, scale, _ = ops.rms_norm_quant(x.to(dev), gamma.to(dev), epsilon=epsilon)
+    codes, scale = codes.cpu(), scale.cpu()
+    epsilon = float(torch.tensor(epsilon))  # as the call takes it
+    s = x.double()
+    y = (s * gamma.double()).abs().amax(-1) / torch.sqrt((s * s).mean(-1) + epsilon)  # (held in fp32)
+    none = (scale == 0) & (y / 127.0 < 2.0 ** -149)  # a scale of 0: the codes do not matter
+    keep = ~none & (y < 3.4e38)
+    assert int(keep.sum()) >= 100 or epsilon >= 1e30
+    assert not bool(scale[keep].isnan().any())
+    assert qo.norm_quant_ok(x[keep], None, gamma, epsilon, codes[keep], scale[keep], None)
