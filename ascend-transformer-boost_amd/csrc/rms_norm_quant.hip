@@ -301,23 +301,33 @@ extern "C" int atbmi_rms_norm_quant(const void *x, const void *residual, const v
         nv *= 2;
     }
     const int64_t threads = ((dim / 8 + nv - 1) / nv + WAVE - 1) / WAVE * WAVE;
-    int4kv::WithFlag(dtype == ATBMI_BF16, [&](auto bf16) {
-        constexpr bool BF16 = decltype(bf16)::value;
-        if (!pieces) {
-            normq::NormPlainKernel<BF16><<<static_cast<unsigned>(rows), normq::THREADS, 0, s>>>(a);
-            return;
-        }
-        int4kv::WithFlag(residual != nullptr, [&](auto res) {
-            constexpr bool RES = decltype(res)::value;
-            const dim3 grid(static_cast<unsigned>(rows)), block(static_cast<unsigned>(threads));
-            switch (nv) {
-            case 1: normq::NormRowKernel<BF16, RES, 1><<<grid, block, 0, s>>>(a); break;
-            case 2: normq::NormRowKernel<BF16, RES, 2><<<grid, block, 0, s>>>(a); break;
-            case 4: normq::NormRowKernel<BF16, RES, 4><<<grid, block, 0, s>>>(a); break;
-            default: normq::NormRowKernel<BF16, RES, 8><<<grid, block, 0, s>>>(a); break;
+    // (a workgroup for each row: more rows than one launch has room for go in several)
+    constexpr int64_t LAUNCH_ROWS = 1 << 21;
+    static_assert(LAUNCH_ROWS * normq::MOST_THREADS < (1LL << 32), "threads of a launch");
+    for (int64_t left = rows; left > 0; left -= LAUNCH_ROWS) {
+        const dim3 grid(static_cast<unsigned>(left < LAUNCH_ROWS ? left : LAUNCH_ROWS)), block(static_cast<unsigned>(threads));
+        int4kv::WithFlag(dtype == ATBMI_BF16, [&](auto bf16) {
+            constexpr bool BF16 = decltype(bf16)::value;
+            if (!pieces) {
+                normq::NormPlainKernel<BF16><<<grid, normq::THREADS, 0, s>>>(a);
+                return;
             }
+            int4kv::WithFlag(residual != nullptr, [&](auto res) {
+                constexpr bool RES = decltype(res)::value;
+                switch (nv) {
+                case 1: normq::NormRowKernel<BF16, RES, 1><<<grid, block, 0, s>>>(a); break;
+                case 2: normq::NormRowKernel<BF16, RES, 2><<<grid, block, 0, s>>>(a); break;
+                case 4: normq::NormRowKernel<BF16, RES, 4><<<grid, block, 0, s>>>(a); break;
+                default: normq::NormRowKernel<BF16, RES, 8><<<grid, block, 0, s>>>(a); break;
+                }
+            });
         });
-    });
-    ATBMI_HIP_CHECK(hipGetLastError());
+        ATBMI_HIP_CHECK(hipGetLastError());
+        a.x += LAUNCH_ROWS * a.xStride;
+        a.residual = a.residual ? a.residual + LAUNCH_ROWS * a.rStride : nullptr;
+        a.residualOut = a.residualOut ? a.residualOut + LAUNCH_ROWS * dim : nullptr;
+        a.out += LAUNCH_ROWS * dim;
+        a.scale += LAUNCH_ROWS;
+    }
     return OK;
 }

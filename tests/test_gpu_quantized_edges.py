@@ -86,3 +86,22 @@ def test_norm_quant_rows_anywhere_in_the_range(ops, dev, gamma_power, epsilon, d
     assert int(keep.sum()) >= 100 or epsilon >= 1e30
     assert not bool(scale[keep].isnan().any())
     assert qo.norm_quant_ok(x[keep], None, gamma, epsilon, codes[keep], scale[keep], None)
+
+
+@pytest.mark.parametrize("rows,dim", [(2 ** 24 + 5, 7), (2 ** 26 + 3, 8)])
+def test_norm_quant_more_rows_than_a_launch_holds(ops, dev, rows, dim):
+    """Rows past 2^32 threads of one launch: every row is written, those around the seams are what they should be."""
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(rows)
+    x = torch.randn((rows, dim), generator=gen, device=dev, dtype=torch.bfloat16)
+    gamma = torch.randn((dim,), generator=gen, device=dev, dtype=torch.bfloat16)
+    scale = torch.full((rows,), -1.0, device=dev)
+    out = torch.full((rows, dim), -128, device=dev, dtype=torch.int8)
+    residual_out = torch.full((rows, dim), -9.0, device=dev, dtype=torch.bfloat16)
+    ops.rms_norm_quant(x, gamma, residual=x, out=out, scale=scale, residual_out=residual_out)
+    assert bool((scale >= 0).all()) and bool((out > -128).all()) and torch.equal(residual_out, x + x)
+    seams = torch.arange(0, rows, 2 ** 21)
+    for first in [0, rows - 64] + (seams[1:] - 32).tolist():
+        part = slice(first, min(first + 64, rows))
+        assert qo.norm_quant_ok(x[part].cpu(), x[part].cpu(), gamma.cpu(), 1e-5, out[part].cpu(), scale[part].cpu(),
+                                residual_out[part].cpu())
