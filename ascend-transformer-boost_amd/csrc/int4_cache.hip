@@ -5,6 +5,7 @@
 // Both move a few bytes per value and compute next to nothing: HBM bounds them on long calls and the launch on short
 // ones. In both kernels a lane owns eight channels of a row (16 bytes in the model's type, 4 bytes of codes), D / 8
 // lanes a row, so that rows of the model's type move in 16-byte pieces.
+#include <algorithm>
 #include "pa_internal.h"
 #include "int4_common.h"
 
@@ -432,7 +433,7 @@ extern "C" int atbmi_reshape_and_cache_int4(const void *key, const void *value, 
     const int64_t rowsPerWg = int4kv::MOVE_THREADS / (headDim / 8);
     const int64_t groups = tiles ? (numTokens + int4kv::TILE_TOKENS - 1) / int4kv::TILE_TOKENS * numKvHeads
                                  : (a.numRows + rowsPerWg - 1) / rowsPerWg;
-    if (groups > 0x7fffffffLL) {
+    if (!int4kv::FitsLaunch(groups, int4kv::MOVE_THREADS)) {
         return Fail(ERR_INVALID_PARAM, "reshape_and_cache_int4: %lld rows are more than one launch takes",
                     (long long)a.numRows);
     }
@@ -482,13 +483,13 @@ extern "C" int atbmi_paged_cache_load_int4(const uint8_t *keyCache, const uint8_
                                            "boundaries");
         }
     }
-    // (no sequence is longer than the table's reach)
-    const int64_t longest = maxSeqLen < maxBlocksPerSeq * blockSize ? maxSeqLen : maxBlocksPerSeq * blockSize;
+    // (no sequence is longer than the table's reach, and tokens past the output's rows have no place to go)
+    const int64_t longest = std::min({maxSeqLen, maxBlocksPerSeq * blockSize, outRows});
     const int64_t perWg = 16LL * (WAVE / (headDim / 8));
     const int64_t chunks = (longest + 15 + perWg - 1) / perWg; // (a sequence may begin 15 places into its first group)
-    if (batch > 65535 || numKvHeads > 65535) {
-        return Fail(ERR_INVALID_PARAM, "paged_cache_load_int4: %lld sequences with %lld heads are more than one launch takes",
-                    (long long)batch, (long long)numKvHeads);
+    if (batch > 65535 || numKvHeads > 65535 || !int4kv::FitsLaunch(2 * chunks, WAVE)) {
+        return Fail(ERR_INVALID_PARAM, "paged_cache_load_int4: %lld sequences of %lld tokens with %lld heads are more than one "
+                                       "launch takes", (long long)batch, (long long)longest, (long long)numKvHeads);
     }
     int4kv::LoadArgs a{};
     a.keyCache = keyCache;

@@ -110,6 +110,12 @@ inline int CheckCache(const char *who, int32_t dtype, int64_t numKvHeads, int64_
     return OK;
 }
 
+// A launch has fewer than 2^32 threads along each dimension of its grid.
+inline bool FitsLaunch(int64_t workgroups, int64_t threads)
+{
+    return workgroups <= 0xffffffffLL / threads;
+}
+
 // Compile-time values from run-time ones.
 template <typename F> void WithFlag(bool flag, F &&next)
 {

@@ -779,6 +779,12 @@ int Check(int64_t m, int64_t n, int64_t k)
     return OK;
 }
 
+int TooLarge(int64_t m, int64_t n)
+{
+    return Fail(ERR_INVALID_PARAM, "linear_int8: %lld tokens by %lld channels are more than one launch takes", (long long)m,
+                (long long)n);
+}
+
 } // namespace lin8
 } // namespace atbmi
 
@@ -854,6 +860,10 @@ extern "C" int atbmi_linear_int8(const int8_t *x, const int8_t *w, const float *
                 const dim3 grid(static_cast<unsigned>((n + 16 * plan.ct - 1) / (16 * plan.ct)), splits,
                                 static_cast<unsigned>((m + 16 * plan.mt - 1) / (16 * plan.mt)));
                 constexpr int MT = decltype(mt)::value, CT = decltype(ct)::value;
+                if (!int4kv::FitsLaunch(grid.x, lin8::SKINNY_WAVES * WAVE)) {
+                    rc = lin8::TooLarge(m, n);
+                    return;
+                }
                 auto kernel = lin8::LinearSkinnyKernel<MT, CT, VEC>;
                 rc = ConfigureKernelLds(reinterpret_cast<const void *>(kernel), lin8::SkinnyLds<MT, CT>());
                 if (rc == OK) {
@@ -878,8 +888,8 @@ extern "C" int atbmi_linear_int8(const int8_t *x, const int8_t *w, const float *
         }
         auto launch = [&](auto kernel, int tn, int tm, int threads, int ldsBytes) {
             const int64_t tilesN = (n + tn - 1) / tn, tilesM = (m + tm - 1) / tm;
-            if (tilesN * tilesM > 0x7fffffffLL) {
-                rc = Fail(ERR_INVALID_PARAM, "linear_int8: %lld tiles", (long long)(tilesN * tilesM));
+            if (!int4kv::FitsLaunch(tilesN * tilesM, threads)) {
+                rc = lin8::TooLarge(m, n);
                 return;
             }
             rc = ConfigureKernelLds(reinterpret_cast<const void *>(kernel), ldsBytes);

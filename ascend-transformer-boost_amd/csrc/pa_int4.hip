@@ -991,8 +991,11 @@ extern "C" int atbmi_pa_int4_decode(const AtbmiPaInt4Call *call, void *workspace
     }
     const int64_t grid = shape.ranges * shape.pairs;
     const int64_t mergeGrid = shape.pairs * call->batch;
-    if (grid > 0x7fffffffLL || mergeGrid > 0x7fffffffLL) {
-        return Fail(ERR_INVALID_PARAM, "pa_int4: %lld workgroups", (long long)std::max(grid, mergeGrid));
+    // (many ranges a sequence: many parts to join for each)
+    const int mergeThreads = shape.ranges > 4 * static_cast<int64_t>(call->batch) ? int4kv::MERGE_MOST_THREADS : 256;
+    if (!int4kv::FitsLaunch(grid, int4kv::PA_THREADS) || (shape.merge && !int4kv::FitsLaunch(mergeGrid, mergeThreads))) {
+        return Fail(ERR_INVALID_PARAM, "pa_int4: %d sequences with %lld groups of 16 query rows are more than one launch takes",
+                    call->batch, (long long)shape.pairs);
     }
     int4kv::PaInt4Args a{};
     a.q = static_cast<const uint16_t *>(call->query);
@@ -1063,9 +1066,7 @@ extern "C" int atbmi_pa_int4_decode(const AtbmiPaInt4Call *call, void *workspace
             if (hipError_t e = hipGetLastError(); e != hipSuccess) {
                 rc = Fail(ERR_RT_FAIL, "pa_int4: launch failed: %s", hipGetErrorString(e));
             } else if (shape.merge) {
-                // (many ranges a sequence: many parts to join for each)
-                const int threads = shape.ranges > 4 * static_cast<int64_t>(call->batch) ? int4kv::MERGE_MOST_THREADS : 256;
-                int4kv::PaInt4MergeKernel<D, BF16><<<static_cast<unsigned>(mergeGrid), threads, 0, s>>>(a);
+                int4kv::PaInt4MergeKernel<D, BF16><<<static_cast<unsigned>(mergeGrid), mergeThreads, 0, s>>>(a);
             }
         });
     });

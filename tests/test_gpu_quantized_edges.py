@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import quant_oracle as qo
-from test_gpu_quantized import DTYPES, _gen, _randn
+from test_gpu_quantized import DTYPES, _gen, _random_cache, _randn
 
 pytestmark = pytest.mark.gpu
 
@@ -105,3 +105,16 @@ def test_norm_quant_more_rows_than_a_launch_holds(ops, dev, rows, dim):
         part = slice(first, min(first + 64, rows))
         assert qo.norm_quant_ok(x[part].cpu(), x[part].cpu(), gamma.cpu(), 1e-5, out[part].cpu(), scale[part].cpu(),
                                 residual_out[part].cpu())
+
+
+def test_load_with_the_widest_table(ops, dev):
+    """A table that reaches almost 2^30 positions and no bound on the lengths: the launch follows the rows there are."""
+    gen = _gen(31)
+    cache = _random_cache(ops, gen, 4, 1, 16, 256, torch.bfloat16, dev)
+    tables = torch.full((1, 2 ** 26 - 1), -1, dtype=torch.int32, device=dev)
+    tables[0, :4] = torch.tensor([2, 0, 3, 1], dtype=torch.int32, device=dev)
+    lens = torch.tensor([61], dtype=torch.int32, device=dev)
+    got = ops.paged_cache_load_int4(*cache, tables, lens, 50)
+    want = ops.paged_cache_load_int4(*cache, tables[:, :4].contiguous(), lens, 61)
+    for a, b in zip(got, want):
+        assert a.shape == (50, 1, 256) and torch.equal(a, b[:50])
