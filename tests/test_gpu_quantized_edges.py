@@ -4,7 +4,8 @@ import pytest
 import torch
 
 import quant_oracle as qo
-from test_gpu_quantized import DTYPES, _gen, _random_cache, _randn
+from test_gpu_quantized import DTYPES, _attention_case, _check_attention, _gen, _mask, _random_cache, _randn
+from test_gpu_quantized_cut import _wide
 
 pytestmark = pytest.mark.gpu
 
@@ -118,3 +119,45 @@ def test_load_with_the_widest_table(ops, dev):
     want = ops.paged_cache_load_int4(*cache, tables[:, :4].contiguous(), lens, 61)
     for a, b in zip(got, want):
         assert a.shape == (50, 1, 256) and torch.equal(a, b[:50])
+
+
+LARGE = [
+    # lens, heads, kv_heads, d, block, tokens, cut
+    ([1, 300, 40], 4, 1, 128, 16, 1, False),
+    ([700, 65], 8, 1, 64, 64, 1, False),
+    ([129, 400], 4, 1, 256, 32, 4, False),
+    ([2100, 30, 0, 900], 8, 2, 128, 128, 1, True),
+    ([640, 1700], 8, 1, 128, 64, 1, True),
+    ([1500, 200], 4, 1, 256, 16, 5, True),
+    ([900, 1100, 3], 4, 2, 64, 128, 2, True),
+]
+
+
+@pytest.mark.parametrize("mask", [None, "-inf"])
+@pytest.mark.parametrize("power", [88, 96, 112, 124])
+@pytest.mark.parametrize("lens,heads,kv_heads,d,block,tokens,cut", LARGE)
+def test_attention_over_the_largest_bf16_values(ops, dev, lens, heads, kv_heads, d, block, tokens, cut, power, mask):
+    """Value rows up to the type's largest numbers, whose weighted sums leave fp32: the means are finite and as near as
+    elsewhere, in one sequence of the batch; the others keep every bit."""
+    gen = _gen(sum(lens) + d)
+    query, cache, tables, n, scale = _attention_case(ops, dev, gen, lens, heads, kv_heads, d, block, torch.bfloat16, tokens)
+    if cut:
+        tables = _wide(tables, block)
+    m = None if mask is None else _mask(gen, mask, len(lens), heads, tokens, max(lens), torch.bfloat16)
+    before = _check_attention(ops, dev, query, cache, tables, n, scale, tokens, block, m)
+    own = tables[1][: -(-lens[1] // block)].long().to(dev)
+    cache[3][own] *= 2.0 ** power
+    got = _check_attention(ops, dev, query, cache, tables, n, scale, tokens, block, m)
+    assert bool(got.isfinite().all())
+    rows = torch.arange(len(lens)).repeat_interleave(tokens)
+    assert torch.equal(got[rows != 1], before[rows != 1])
+
+
+@pytest.mark.parametrize("length", [5, 1024, 3000])
+def test_attention_over_rows_of_the_largest_number(ops, dev, length):
+    """Every value is the largest bf16 number: so is the mean."""
+    gen = _gen(length)
+    query, cache, tables, n, scale = _attention_case(ops, dev, gen, [length], 4, 1, 128, 128, torch.bfloat16, 1)
+    cache[3][..., 0], cache[3][..., 1] = 0.0, torch.finfo(torch.bfloat16).max
+    got = _check_attention(ops, dev, query, cache, tables, n, scale, 1, 128)
+    assert bool((got == torch.finfo(torch.bfloat16).max).all())
