@@ -549,13 +549,31 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
                 }
             }
             if constexpr (MASK) {
+                // The largest bf16 values leave fp32 when they are turned into log2 units. From LARGE on they grow by half
+                // instead (a tile that has any takes that branch): still apart by far more than scores are, and in the same
+                // order, and a row of nothing but the lowest value is the mean of its values.
+                constexpr float LARGE = 0x1p126f;
+                bool large = false;
+                if constexpr (BF16) {
 #pragma unroll
-                for (int j = 0; j < NC; ++j) {
-                    // (the lowest finite value leaves fp32 when it is turned into log2 units: it stays finite here, so that
-                    // a row of nothing else is the mean of its values; NaN stays NaN)
-                    float v = __builtin_fmaf(bias[j], LOG2E, s[j]);
-                    v = v < -3.0e38f ? -3.0e38f : v;
-                    s[j] = bias[j] == -INFINITY ? -INFINITY : v;
+                    for (int j = 0; j < NC; ++j) {
+                        large |= fabsf(bias[j]) > LARGE && bias[j] != -INFINITY;
+                    }
+                }
+                if (BF16 && __ballot(large) != 0) {
+#pragma unroll
+                    for (int j = 0; j < NC; ++j) {
+                        const bool slow = fabsf(bias[j]) > LARGE;
+                        const float from = slow ? __builtin_copysignf(LARGE * (LOG2E - 0.5f), bias[j]) : 0.0f;
+                        const float v = __builtin_fmaf(bias[j], slow ? 0.5f : LOG2E, s[j] + from);
+                        s[j] = bias[j] == -INFINITY ? -INFINITY : v;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < NC; ++j) {
+                        const float v = __builtin_fmaf(bias[j], LOG2E, s[j]);
+                        s[j] = bias[j] == -INFINITY ? -INFINITY : v;
+                    }
                 }
             }
             if constexpr (HIDDEN) {

@@ -1,5 +1,7 @@
 """The quantised decoder-layer operators at the edges of what their definition allows, against 64-bit plain implementations:
 outputs that only the C ABI offers, values at the ends of the types' ranges, launches of many rows."""
+import math
+
 import pytest
 import torch
 
@@ -161,3 +163,21 @@ def test_attention_over_rows_of_the_largest_number(ops, dev, length):
     cache[3][..., 0], cache[3][..., 1] = 0.0, torch.finfo(torch.bfloat16).max
     got = _check_attention(ops, dev, query, cache, tables, n, scale, 1, 128)
     assert bool((got == torch.finfo(torch.bfloat16).max).all())
+
+
+@pytest.mark.parametrize("heads,d,block,tokens,cut", [(4, 128, 128, 1, False), (8, 64, 16, 1, False), (8, 256, 32, 2, True), (4, 128, 64, 1, True)])
+def test_attention_masks_of_the_largest_numbers(ops, dev, heads, d, block, tokens, cut):
+    """Different masks of the bf16 type's largest numbers, of either sign: positions under the highest of a row share it, the
+    others have no part in it."""
+    gen = _gen(heads + d)
+    big = torch.finfo(torch.bfloat16).max
+    lens = [150, 64, 7, 201, 333, 90]
+    query, cache, tables, n, scale = _attention_case(ops, dev, gen, lens, heads, 1, d, block, torch.bfloat16, tokens)
+    low = torch.tensor([-big, -0.97 * big, -0.9 * big, -0.5 * big, -0.3 * big, -math.inf])
+    mask = torch.empty((len(lens), 1, 1, max(lens)))
+    for b, chosen in enumerate(([0, 1], [0, 1, 2, 5], [2, 3], [0, 4, 5], [0, 5])):
+        mask[b, 0, 0] = low[chosen][torch.randint(0, len(chosen), (max(lens),), generator=gen)]
+    mask[5, 0, 0] = (torch.rand((max(lens),), generator=gen) < 0.3).float() * big - big * (torch.arange(max(lens)) % 2)
+    mask = mask.to(torch.bfloat16)
+    got = _check_attention(ops, dev, query, cache, _wide(tables, block) if cut else tables, n, scale, tokens, block, mask)
+    assert bool(got.isfinite().all())
