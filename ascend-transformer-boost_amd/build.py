@@ -2,7 +2,8 @@
 
   lib/libatbmi_kernels.so  HIP kernels + C ABI (hipcc, --offload-arch=gfx950)
   lib/libatb.so            atb::Operation layer + flat C view (g++), links the first
-  lib/quantized_ext.so     the calls of quantized.py on torch tensors (g++), links torch and the first
+  lib/quantized_ext.so     the calls of quantized.py on torch tensors (g++), links torch and the first; left out, with a note,
+                           where torch or Python's headers are not installed
 
 hipcc cross-compiles gfx950 code objects without a GPU, so this runs anywhere
 the ROCm toolchain is installed. Usage: python3 build.py [--jobs N] [--sanitize]
@@ -82,6 +83,17 @@ def build_host():
     return target
 
 
+def torch_ext_lacks():
+    """What build_torch_ext needs and this machine has not; None if it has everything."""
+    import importlib.util
+    import sysconfig
+    if importlib.util.find_spec("torch") is None:
+        return "torch"
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        return "Python's headers"
+    return None
+
+
 def build_torch_ext():
     """The extension module behind quantized.py (host code only; torch's headers want to know the HIP platform)."""
     import sysconfig
@@ -112,10 +124,16 @@ def build_tools():
 
 
 def build_all(jobs=8):
-    with concurrent.futures.ThreadPoolExecutor(max_workers=2) as pool:
-        kernels = build_kernels(jobs)
-        ext = pool.submit(build_torch_ext)
-        return [kernels, build_host(), ext.result(), build_tools()]
+    with concurrent.futures.ThreadPoolExecutor(max_workers=1) as pool:
+        built = [build_kernels(jobs)]
+        lacks = torch_ext_lacks()
+        ext = pool.submit(build_torch_ext) if lacks is None else None
+        built += [build_host(), build_tools()]
+        if ext is None:
+            print("quantized_ext.so is not built (quantized.py needs it): %s not found" % lacks)
+        else:
+            built.append(ext.result())  # (a failure is raised when the rest is there)
+        return built
 
 
 def sanitizer_runtime():
