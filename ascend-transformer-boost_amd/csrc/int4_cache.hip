@@ -314,7 +314,7 @@ __global__ __launch_bounds__(WAVE) void LoadKernel(const LoadArgs a)
     const int b = blockIdx.y;
     const int g = blockIdx.z;
     const int l = lane % LPR;
-    const int start = a.starts ? max(a.starts[b], 0) : 0;
+    const int start = a.starts ? a.starts[b] : 0;
     const int len = min(a.lens[b], a.maxSeqLen);
     const int64_t pos0 = (static_cast<int64_t>(start) & ~15LL) + (static_cast<int64_t>(blockIdx.x / 2) * GROUPS + lane / LPR) * 16;
     const int64_t end = static_cast<int64_t>(start) + len;
@@ -325,7 +325,7 @@ __global__ __launch_bounds__(WAVE) void LoadKernel(const LoadArgs a)
     if (pos0 >= end) {
         return;
     }
-    if (pos0 >= static_cast<int64_t>(a.maxBlocksPerSeq) * a.blockSize) { // (that is below 2^30)
+    if (pos0 < 0 || pos0 >= static_cast<int64_t>(a.maxBlocksPerSeq) * a.blockSize) { // (that is below 2^30)
         return;
     }
     const int tableAt = static_cast<int>(pos0) / a.blockSize;

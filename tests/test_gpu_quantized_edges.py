@@ -181,3 +181,29 @@ def test_attention_masks_of_the_largest_numbers(ops, dev, heads, d, block, token
     mask = mask.to(torch.bfloat16)
     got = _check_attention(ops, dev, query, cache, _wide(tables, block) if cut else tables, n, scale, tokens, block, mask)
     assert bool(got.isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("d", [64, 256])
+def test_load_from_positions_in_front_of_the_first(ops, dev, d, dtype):
+    """A start below zero: the positions in front of the sequence have no row, their places stay as they are, and the others lie
+    where they would."""
+    gen = _gen(d)
+    cache = _random_cache(ops, gen, 6, 2, 16, d, dtype, dev)
+    tables = torch.tensor([[3, 1, 4], [0, 5, 2], [1, 2, 3], [4, 0, 5]], dtype=torch.int32, device=dev)
+    starts, lens = [-5, -16, -2 ** 31, 2], [30, 20, 25, 7]
+    rows = sum(lens)
+    key = torch.full((rows, 2, d), 9.0, dtype=dtype, device=dev)
+    value = torch.full((rows, 2, d), -9.0, dtype=dtype, device=dev)
+    put = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    ops.paged_cache_load_int4(*cache, tables, put(lens), rows, seq_starts=put(starts), key=key, value=value)
+    all_rows = ops.paged_cache_load_int4(*cache, tables, put([48] * 4), 4 * 48)
+    for got, full, empty in ((key, all_rows[0], 9.0), (value, all_rows[1], -9.0)):
+        want = torch.full_like(got, empty)
+        at = 0
+        for b in range(4):
+            for t in range(lens[b]):
+                if starts[b] + t >= 0:
+                    want[at + t] = full[48 * b + starts[b] + t]
+            at += lens[b]
+        assert torch.equal(got, want)
