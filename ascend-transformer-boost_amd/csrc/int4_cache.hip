@@ -152,7 +152,7 @@ __global__ __launch_bounds__(MOVE_THREADS) void WriteKernel(const WriteArgs a)
 // The same for many tokens: a workgroup takes 64 tokens of one head, a wave 16 of them. Value codes lie token after token in
 // the cache, so they are turned in LDS: a wave then stores 64 neighbouring tokens' bytes of one channel pair at a time,
 // which the memory takes as one piece where the tokens' slots follow each other (as a prompt's do) and byte by byte where
-// they do not. (2048 new tokens of 5 sequences with 8 heads of 128 channels: 40 -> 17 us, against bytes stored from
+// they do not. (2048 new tokens of 5 sequences with 8 heads of 128 channels: 40 -> 16 us, against bytes stored from
 // the lanes of the row; one token a call of 512 sequences: 7 us in rows, 11 us in tiles, so that fewer than 1024 go in rows.)
 constexpr int TILE_TOKENS = 64;
 constexpr int TILE_FROM = 1024;

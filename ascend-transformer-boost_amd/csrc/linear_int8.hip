@@ -516,9 +516,10 @@ __global__ __launch_bounds__(RING_WAVES *WAVE, 2) void LinearRingKernel(const Ar
 // A workgroup of eight waves takes 16 CT channels and all tokens (16 MT of them; fewer are padded by repeating the last).
 // The waves take the 128-value chunks of the contraction in turn, each through LDS of its own (RING chunks of rows of 128
 // bytes, eight an instruction, piece p of row r at place p ^ (r % 8): whole cache lines from memory, which is what bounds
-// this kernel; with 64-byte rows 64 x 6144 x 4096 took 13.8 us instead of 11.1), and join their integer sums at the end: no barrier in between. What is read of the activations
-// comes from L2, MT / CT times the weights' bytes. (Straight into registers in the matrix instruction's layout, 16
-// neighbouring lanes read 16 bytes of 16 rows each: 64 tokens by 6144 channels by 4096 took 24 us that way.)
+// this kernel; with 64-byte rows 64 x 6144 x 4096 took 13.8 us instead of 11.1, its weights from HBM), and join their
+// integer sums at the end: no barrier in between. What is read of the activations comes from L2, MT / CT times the
+// weights' bytes. (Straight into registers in the matrix instruction's layout, 16 neighbouring lanes read 16 bytes of 16
+// rows each: 64 tokens by 6144 channels by 4096 took 24 us that way.)
 constexpr int SKINNY_WAVES = 8;
 template <int MT, int CT> constexpr int SkinnyRing()
 {
@@ -546,11 +547,10 @@ __global__ __launch_bounds__(SKINNY_WAVES *WAVE, 1) void LinearSkinnyKernel(cons
     const int c = lane & 15;
     const int kg = lane >> 4;
     const int n0 = blockIdx.x * 16 * CT;
-    const int m0 = blockIdx.z * 16 * MT;
     const int kBegin = blockIdx.y * sp.kPer;
     const int kEnd = min(a.k, kBegin + sp.kPer);
     const int8_t *wBase = a.w + static_cast<int64_t>(n0) * a.wStride;
-    const int8_t *xBase = a.x + static_cast<int64_t>(m0) * a.xStride;
+    const int8_t *xBase = a.x;
     unsigned char *mine = lds + wave * RING * CHUNK;
     const int chunk16 = 16 * ((lane % 8) ^ (lane / 8));
     uint32_t at[MOVES]; // instruction i: rows 8 i .. + 7 (weights, then tokens)
@@ -558,7 +558,7 @@ __global__ __launch_bounds__(SKINNY_WAVES *WAVE, 1) void LinearSkinnyKernel(cons
     for (int i = 0; i < MOVES; ++i) {
         const bool isW = i < 2 * CT;
         const int row = 8 * (isW ? i : i - 2 * CT) + lane / 8;
-        const int r = isW ? min(row, a.n - 1 - n0) : min(row, a.m - 1 - m0);
+        const int r = isW ? min(row, a.n - 1 - n0) : min(row, a.m - 1);
         at[i] = static_cast<uint32_t>(r) * static_cast<uint32_t>(isW ? a.wStride : a.xStride) + chunk16;
     }
     i32x4 acc[CT][MT];
@@ -672,7 +672,7 @@ __global__ __launch_bounds__(SKINNY_WAVES *WAVE, 1) void LinearSkinnyKernel(cons
             sum += joined[(v * CT * MT + f) * WAVE + lane];
         }
         const int n = n0 + 16 * (f / MT) + 4 * kg;
-        const int m = m0 + 16 * (f % MT) + c;
+        const int m = 16 * (f % MT) + c;
         if (m < a.m && n < a.n) {
             if (sp.partial) {
                 StorePartial(a, sp.partial + (static_cast<int64_t>(blockIdx.y) * a.m + m) * a.n + n, n, sum);
@@ -722,10 +722,11 @@ struct Plan {
 
 // The cheapest by measured times (us, MI355X). A workgroup of any kind fills a CU, so a kernel costs the rounds that its
 // workgroups make on the CUs times what one takes for its part kPer of the contraction:
-//   256 x 256   5 + 0.0137 kPer     (64 x 64 tiles of 8192: 459; 24 x 8 tiles of 4096, one round: 62)
+//   256 x 256   5 + 0.0137 kPer     (32 x 32 tiles of 8192, four rounds: 459; 24 x 8 tiles of 4096, one round: 62)
 //   128 x 128   3 + 0.0061 kPer     (48 x 4 tiles of 4096, one round: 28; 48 x 16, three rounds: 78)
 //   few tokens  2.5 + rounds kPer x {0.0011, 0.0013, 0.0014} (one channel tile and 16, 32, 64 tokens),
-//               {0.0013, 0.0015, 0.0019} (two)   (64 x 6144 x 4096, one round: 11; 64 x 10240 x 8192, two: 33)
+//               {0.0013, 0.0015, 0.0019} (two)   (64 x 6144 x 4096, one round: 11; 64 x 10240 x 8192, a round and a
+//               quarter that counts as two, 34: 25; all with weights from HBM)
 // and splitting the contraction 4 us and 0.2 a part for the kernel that joins the parts and their bytes at 4 TB/s (128 x 6144 x 4096:
 // 29 whole, 18 in four parts; 512 x 6144 x 4096: 28 whole, 43 in two).
 Plan PlanOf(int64_t m, int64_t n, int64_t k)
@@ -857,8 +858,7 @@ extern "C" int atbmi_linear_int8(const int8_t *x, const int8_t *w, const float *
         constexpr bool VEC = decltype(v)::value;
         if (plan.kind == lin8::SKINNY) {
             auto launch = [&](auto mt, auto ct) {
-                const dim3 grid(static_cast<unsigned>((n + 16 * plan.ct - 1) / (16 * plan.ct)), splits,
-                                static_cast<unsigned>((m + 16 * plan.mt - 1) / (16 * plan.mt)));
+                const dim3 grid(static_cast<unsigned>((n + 16 * plan.ct - 1) / (16 * plan.ct)), splits);
                 constexpr int MT = decltype(mt)::value, CT = decltype(ct)::value;
                 if (!int4kv::FitsLaunch(grid.x, lin8::SKINNY_WAVES * WAVE)) {
                     rc = lin8::TooLarge(m, n);

@@ -22,7 +22,7 @@
 //   values   O^T = V^T P^T: A = value codes, which lie token after token (16 tokens of a channel pair are 16 bytes: a
 //            lane's tokens 16 kg .. + 15), B = the lane's own 16 weights. With 16 columns the weights stay in the lane
 //            that has the scores; with fewer, scores and weights pass through LDS once so that no lane computes the
-//            softmax of a repeated column (batch of 64, 4 columns, 1024 to 4096 tokens: 54 -> 50 us).
+//            softmax of a repeated column (batch of 64, 4 columns, 1024 to 4096 tokens: 49.5 -> 47.8 us).
 // Running maximum and sums are fp32. The maximum a column is scaled by moves only when a score exceeds it by more
 // than 2^8 (in the exponent: 8): weights up to 256 are as exact as weights up to 1, and the accumulators are rescaled
 // a few times a context instead of every tile.
@@ -129,8 +129,8 @@ __device__ __forceinline__ int WaveSum(int v)
 
 // What is cut into ranges: the tiles of a sequence behind START units that stand for none. They are what a sequence costs
 // a workgroup beyond its tiles (its first tiles are waited for, its sums are joined), so that equal ranges take equally
-// long. (19 sequences of 256 .. 32768 with 16 columns: 51.0 us with 2, 48.9 with 4, 46.1 with 8 and 11; 64 sequences of
-// 1024 .. 4096 with 4 columns: 50.1, 49.9, 49.0 and 50.1.)
+// long. (19 sequences of 256 .. 32768 with 16 columns: 49.2 us with 2, 46.8 with 4, 43.9 with 8, 44.0 with 11; 64 sequences
+// of 1024 .. 4096 with 4 columns: 49.1, 48.6, 47.8 and 47.7.)
 __device__ __forceinline__ int UnitsOf(int len)
 {
     return TilesOf(len) + START;
@@ -145,11 +145,6 @@ __device__ __forceinline__ int RangeBegin(int r, int units, int live)
     return static_cast<int>(static_cast<int64_t>(units) * r / live);
 }
 
-__device__ __forceinline__ float QuadMax(float x)
-{
-    x = fmaxf(x, __shfl_xor(x, 16));
-    return fmaxf(x, __shfl_xor(x, 32));
-}
 __device__ __forceinline__ float QuadSum(float x)
 {
     x += __shfl_xor(x, 16);
@@ -194,7 +189,7 @@ __device__ __forceinline__ uint32_t PackBf16(float a, float b)
 // 16 bytes (4 bytes) a lane to LDS at ldsAt + 16 (4) x lane, from an address of its own or from an offset to the wave's;
 // read once, so not to displace anything. Value codes in long blocks are left in the L2 a while (Kept): a 64-token tile takes
 // half of each 128-byte line of theirs, and the wave that takes the other half comes about the same time (fp16, batch of 128 with
-// 2048 .. 8192 tokens: 172 -> 165 us, keys without the hint as well: 185 us; with 64 and 256 channels 3 % slower).
+// 2048 .. 8192 tokens: 156 -> 149 us, and slower again with the keys kept as well; with 64 and 256 channels 3 % slower).
 __device__ __forceinline__ void ToLds16(const void *from, uint32_t ldsAt)
 {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(ldsAt), "v"(from) : "memory", "m0");

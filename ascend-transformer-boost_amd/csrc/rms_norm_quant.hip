@@ -290,7 +290,7 @@ extern "C" int atbmi_rms_norm_quant(const void *x, const void *residual, const v
                         normq::Aligned(residual, 16) && normq::Aligned(gamma, 16) && normq::Aligned(residualOut, 16) &&
                         normq::Aligned(out, 8);
     // Threads a row. Few rows leave CUs idle, so each gets a thread for every piece. Many rows fill the chip with small
-    // workgroups of up to four pieces a thread (8191 x 8192 with a residual: 83 us, 5.7 TB/s), larger ones only where a row
+    // workgroups of up to four pieces a thread (8191 x 8192 with a residual: 72 us, 6.5 TB/s), larger ones only where a row
     // has more.
     int64_t most = rows < 2LL * DeviceComputeUnits() ? normq::MOST_THREADS : normq::THREADS;
     while (most < normq::MOST_THREADS && dim / 8 > most * 4) {
