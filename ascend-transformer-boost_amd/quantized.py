@@ -9,7 +9,8 @@
 
 Each function checks its arguments (ValueError), launches the HIP kernel through the C ABI (include/atbmi_kernels.h, which
 defines the operators) on torch's current stream of the tensors' device, and returns without waiting; a failure of the
-launch raises RuntimeError. Nothing is read back from the device, so all of them can be captured into a HIP graph; results
+launch raises RuntimeError, as do tensors without memory of their own (those of torch.vmap). The functions have no gradients.
+Nothing is read back from the device, so all of them can be captured into a HIP graph; results
 and workspaces come from torch's allocator unless they are handed in (`out=` and its like).
 
 The calls themselves are made by an extension module (torch_ext/quantized_ext.cpp). It does nothing and returns None when an
@@ -94,7 +95,8 @@ def paged_attention_int4(query, key_cache, value_cache, key_params, value_params
     """Attention of query [batch * query_tokens, heads, head_dim] over a 4-bit cache; query token j of a sequence sees its
     first context_lens[b] - query_tokens + 1 + j positions. mask, in the query's type and [batch | 1, heads | 1,
     query_tokens | 1, positions] with positions next to each other, is added to the scaled scores; positions past its
-    length are hidden. `workspace`: a uint8 tensor to use instead of a new one."""
+    length are hidden. `workspace`: a uint8 tensor to use instead of a new one. Tables that reach much further than the
+    contexts cost short ones a few microseconds (see AtbmiPaInt4Call)."""
     got = (_module or _ext()).paged_attention_int4(query, key_cache, value_cache, key_params, value_params, block_tables,
                                                    context_lens, qk_scale, query_tokens, mask, out, workspace)
     return got if got is not None else _refuse_attention(query, (key_cache, value_cache, key_params, value_params),

@@ -662,8 +662,9 @@ int atbmi_mla_mask_free_expand(const AtbmiMlaMaskFreeCall *call, void *workspace
  * A row with a value (or gamma with one) that is not finite gets scale NaN and codes 0. Rows of finite values may lie anywhere
  * in dtype's range, and epsilon anywhere in fp32's; only a row whose products s * gamma all lie below 2^-118, also with s
  * multiplied by the power of two that brings its largest value between a half and one, counts as zeros. x and residual have
- * row strides of their own (elements, >= dim); out and residualOut are [rows, dim] without gaps. residualOut may be x or residual itself
- * when that has no gaps either. dtype (fp16 or bf16) is the type of x, residual, gamma and residualOut; dim <= 65536.
+ * row strides of their own (elements, >= dim); out and residualOut are [rows, dim] without gaps. residualOut may be x or
+ * residual itself when that has no gaps either. dtype (fp16 or bf16) is the type of x, residual, gamma and residualOut;
+ * dim <= 65536, rows < 2^31.
  */
 int atbmi_rms_norm_quant(const void *xDevice, const void *residualDevice, const void *gammaDevice, int8_t *outDevice,
                          float *scaleDevice, void *residualOutDevice, int64_t rows, int64_t dim, int64_t xRowStride,
@@ -701,7 +702,7 @@ int atbmi_linear_int8(const int8_t *xDevice, const int8_t *wDevice, const float 
  * s = slotMapping[i] (block s / blockSize, place s % blockSize); a slot outside [0, numBlocks * blockSize) skips the
  * token. With hi and lo the largest and smallest value of the row, scale = (hi - lo) / 15 and middle = (hi + lo) / 2,
  * rounded to dtype, and code = rint((x - middle) / scale + 7.5) in [0, 15] (scale 0: code 8, so the row stands for its
- * middle). A row with a value that is not finite gets scale and middle NaN. key and value are [numTokens, numKvHeads,
+ * middle). Ties go to the even code, and a place within 2^-18 of the middle between two codes counts as a tie. A row with a value that is not finite gets scale and middle NaN. key and value are [numTokens, numKvHeads,
  * D] with a token stride of their own (elements, >= numKvHeads * D): slices of a fused projection's output need no
  * copy. The slots of one call must differ: of a slot named twice the content is undefined.
  */
@@ -716,7 +717,8 @@ int atbmi_reshape_and_cache_int4(const void *keyDevice, const void *valueDevice,
  * sequence (seqStarts NULL: 0; a position of its own, not a block's), found in block blockTables[b][p / blockSize],
  * and lands in row (tokens of the sequences before b) + t of key and value, dtype [outRows, numKvHeads, D] without
  * gaps, 16-byte aligned. Left untouched: rows of positions outside the table or in blocks outside [0, numBlocks), and
- * what lies at or past outRows. A length below zero counts as zero. maxSeqLen bounds the lengths (the launch is sized
+ * what lies at or past outRows (positions in front of the sequence, where a start is below zero, are outside the table). A
+ * length below zero counts as zero. maxSeqLen bounds the lengths (the launch is sized
  * by it): tokens at or past it stay unread, but keep their rows.
  */
 int atbmi_paged_cache_load_int4(const uint8_t *keyCacheDevice, const uint8_t *valueCacheDevice, const void *keyParamsDevice,
@@ -735,7 +737,13 @@ int atbmi_paged_cache_load_int4(const uint8_t *keyCacheDevice, const uint8_t *va
  * Positions in blocks outside [0, numBlocks) are not seen. With a mask (dtype), mask[b * maskSeqStride + h *
  * maskHeadStride + j * maskRowStride + p] (elements; 0: shared) is added to the scaled score; -inf hides the position
  * whatever its score is, and positions at or past maskLen are hidden too. A row that sees nothing is written as zeros.
- * query and out start on 16-byte boundaries.
+ * query and out start on 16-byte boundaries. Scores, softmax and sums are fp32; the weights that meet the value codes are
+ * rounded to bf16 for bf16 models and to twice its bits for fp16 models.
+ * maxBlocksPerSeq tells how long a context may be, since the lengths stay on the device: where it allows only short ones
+ * (up to 1024 positions, or 2048 with a workgroup for every CU) a workgroup takes whole sequences, else they are cut and a
+ * second kernel joins the parts, whatever their lengths are. A table as wide as a model's longest context costs a batch of
+ * short ones 3 to 5 us (one sequence of 512: 7.9 us with a table of 512, 12.6 with a wide one; 64 of 1024: 18.6, 21.9), so a
+ * server that captures graphs may keep one of a narrow table beside the wide one's.
  */
 typedef struct AtbmiPaInt4Call {
     int32_t dtype;             /* ATBMI_F16 or ATBMI_BF16: query, mask, params and out */
