@@ -399,7 +399,7 @@ extern "C" int atbmi_reshape_and_cache_int4(const void *key, const void *value, 
     if (int rc = int4kv::CheckCache("reshape_and_cache_int4", dtype, numKvHeads, headDim, blockSize, numBlocks)) {
         return rc;
     }
-    if (numTokens < 0 || keyTokenStride < numKvHeads * headDim || valueTokenStride < numKvHeads * headDim) {
+    if (numTokens < 0 || numTokens > 0x7fffffffLL || keyTokenStride < numKvHeads * headDim || valueTokenStride < numKvHeads * headDim) {
         return Fail(ERR_INVALID_PARAM, "reshape_and_cache_int4: %lld tokens with strides %lld and %lld (rows of %lld)",
                     (long long)numTokens, (long long)keyTokenStride, (long long)valueTokenStride,
                     (long long)(numKvHeads * headDim));
@@ -466,7 +466,7 @@ extern "C" int atbmi_paged_cache_load_int4(const uint8_t *keyCache, const uint8_
     if (int rc = int4kv::CheckCache("paged_cache_load_int4", dtype, numKvHeads, headDim, blockSize, numBlocks)) {
         return rc;
     }
-    if (batch < 0 || maxBlocksPerSeq <= 0 || maxBlocksPerSeq * blockSize >= (1LL << 30) || outRows < 0 || maxSeqLen < 0) {
+    if (batch < 0 || maxBlocksPerSeq <= 0 || maxBlocksPerSeq > ((1LL << 30) - 1) / blockSize || outRows < 0 || maxSeqLen < 0) {
         return Fail(ERR_INVALID_PARAM, "paged_cache_load_int4: batch %lld, %lld blocks a sequence, %lld rows, length %lld",
                     (long long)batch, (long long)maxBlocksPerSeq, (long long)outRows, (long long)maxSeqLen);
     }

@@ -28,3 +28,12 @@ def test_attention_past_a_launch_is_refused(binding):
         call = binding.AtbmiPaInt4Call(**{**PA, **bad})
         assert lib.atbmi_pa_int4_decode(ctypes.byref(call), FAKE, 1 << 62, None) == 1
         assert b"one launch" in lib.atbmi_last_error()
+
+
+@pytest.mark.parametrize("call,good,bad", [
+    ("atbmi_paged_cache_load_int4", LOAD, dict(reach=1 << 60)), ("atbmi_paged_cache_load_int4", LOAD, dict(reach=(1 << 60) + 3)),
+    ("atbmi_paged_cache_load_int4", LOAD, dict(reach=1 << 26)), ("atbmi_reshape_and_cache_int4", WRITE, dict(tokens=1 << 31)),
+    ("atbmi_reshape_and_cache_int4", WRITE, dict(tokens=(1 << 63) - 1, heads=64, ks=1 << 13, vs=1 << 13))])
+def test_counts_whose_products_overflow_are_refused(binding, call, good, bad):
+    lib = binding.kernels()
+    assert getattr(lib, call)(*{**good, **bad}.values()) == 1
