@@ -381,6 +381,9 @@ protected:
             (param_.hasSeqStarts && !Is(in.at(8), {tables.dims[0]}))) {
             return WrongShape(op_, "seqLens and seqStarts [batch], key and value [tokens, heads, headSize] are expected");
         }
+        if (tables.dims[0] > 65535 || cache.dims[1] > 65535 || tables.dims[1] > ((1LL << 30) - 1) / cache.dims[2]) {
+            return WrongShape(op_, "up to 65535 sequences and heads, tables that reach less than 2^30 positions");
+        }
         return NO_ERROR;
     }
     Status InferShapeImpl(const SVector<TensorDesc> &in, SVector<TensorDesc> &out) const override

@@ -674,8 +674,8 @@ int atbmi_rms_norm_quant(const void *xDevice, const void *residualDevice, const 
  * Product of 8-bit integers with a scale for each token and each output channel:
  *   out[i][j] = xScale[i] * wScale[j] * sum_k x[i][k] * w[j][k] + bias[j]
  * x int8 [m, k], w int8 [n, k], xScale fp32 [m], wScale fp32 [n], bias fp32 [n] or NULL, out fp16 / bf16 [m, n], each
- * matrix with a row stride of its own (elements; x and w at most 2^23). The integer sum is exact (k <= 131071 keeps it within 32 bits); it is
- * scaled in fp32 and rounded once. out may not overlap an input.
+ * matrix with a row stride of its own (elements; x and w at most 2^23). The integer sum is exact (k <= 131071 keeps it
+ * within 32 bits); it is scaled in fp32, by the product of the two scales, and rounded once. out may not overlap an input.
  * The workspace (atbmi_linear_int8_workspace_size; its size follows the number of CUs of the current device, so size
  * and launch belong on the same device) holds integer partial sums where the contraction is split; it needs no
  * initial content. Size 0: workspaceDevice may be NULL.

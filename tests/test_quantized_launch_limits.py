@@ -4,7 +4,7 @@ import ctypes
 
 import pytest
 
-from test_quantized_host import FAKE, LINEAR, LOAD, PA, WRITE
+from test_quantized_host import FAKE, LINEAR, LOAD, PA, WRITE, _load, _run
 
 
 @pytest.mark.parametrize("call,good,bad", [
@@ -37,3 +37,12 @@ def test_attention_past_a_launch_is_refused(binding):
 def test_counts_whose_products_overflow_are_refused(binding, call, good, bad):
     lib = binding.kernels()
     assert getattr(lib, call)(*{**good, **bad}.values()) == 1
+
+
+@pytest.mark.parametrize("change", [{4: [70000, 4], 5: [70000], 8: [70000]}, {4: [3, 1 << 25]}])
+def test_load_operation_refuses_what_its_launch_would(binding, change):
+    """In InferShape and Setup, not only when it is executed."""
+    name, param, ins, outs, alias = _load(binding)
+    assert _run(binding, (name, param, ins, outs, alias)) == ("S", "NO_ERROR")
+    ins = [(t, change.get(i, shape)) for i, (t, shape) in enumerate(ins)]
+    assert _run(binding, (name, param, ins, outs, alias)) == ("I", "ERROR_INVALID_TENSOR_DIM")
