@@ -58,9 +58,10 @@ constexpr int START = 8;        // see UnitsOf
 constexpr int WHOLE_TILES = 16; // see ShapeOf
 constexpr float STEP_UP = 8.0f; // how far (log2) a score may exceed the reference before that moves
 // bf16 values may lie so high that the sums leave fp32: weights of up to 2^8 times scales of up to 2^125.1 times operands of up
-// to 31, over up to 2^30 tokens, come to 2^168. Sums that are not below FAR send the range's part of that sequence through once
-// more with its weights brought down by 2^DOWN, which their total shares. (Below FAR, 2^31 parts may be added up. The test costs
-// 0.4 us of 47.4 with a batch of 64 and 0.7 of 43.8 with four query tokens.)
+// to 31, over up to 2^30 tokens, come to 2^168. Columns whose sums are not below FAR are not stored; the range's part of that
+// sequence goes through once more for them, with its weights brought down by 2^DOWN, which their total shares. (Below FAR, 2^31
+// parts may be added up. The others are stored the first time only: `out` may be the query, which is then no longer there. All
+// this costs ordinary rows 0.6 us of 47.4 with a batch of 64 and of 43.8 with four query tokens, 1 % with 64 or 256 channels.)
 constexpr float FAR = 0x1p96f;
 constexpr float DOWN = 48.0f;
 
@@ -262,7 +263,7 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[]; // a ring of tiles for each wave, then sums or masks
     __shared__ float ldsM[PA_WAVES][HT];
     __shared__ float ldsL[PA_WAVES][HT];
-    __shared__ int ldsFar;
+    __shared__ bool ldsFar[HT];
 
     const int lane = threadIdx.x & (WAVE - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
@@ -333,7 +334,7 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
     const int vGrp = (lane % 4) ^ (lane / 8 % 4);
     const uint32_t valueAt = lane / 4 * a.blockSize + 16 * vGrp;
     const int64_t headBytes = static_cast<int64_t>(a.blockSize) * (D / 2);
-    float down = 0.0f; // (bf16 only; see DOWN)
+    float down = 0.0f; // by how much the references lie above the scores that they are taken from (bf16 only: see DOWN)
 
     for (;;) {
         const int len = UniformLen(a, seq);
@@ -585,13 +586,13 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
             for (int j = 1; j < NC; ++j) {
                 most = fmaxf(most, s[j]);
             }
-            if (__ballot(most > top + STEP_UP || (top == -INFINITY && most > -INFINITY)) != 0) {
+            if (__ballot(most > top + (STEP_UP - down) || (top == -INFINITY && most > -INFINITY)) != 0) {
                 float newTop = most;
 #pragma unroll
                 for (int step = NC == 16 ? 16 : 1; step < (NC == 16 ? WAVE : PER); step *= 2) {
                     newTop = fmaxf(newTop, __shfl_xor(newTop, step));
                 }
-                newTop = fmaxf(top, newTop);
+                newTop = fmaxf(top, newTop + down);
                 float keep = top == -INFINITY ? 0.0f : exp2f(top - newTop);
                 top = newTop;
                 total *= keep;
@@ -606,7 +607,7 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
                     acc[i][1] *= keep;
                 }
             }
-            const float base = (top == -INFINITY ? 0.0f : top) + (BF16 ? down : 0.0f);
+            const float base = top == -INFINITY ? 0.0f : top;
             float pv[NC];
 #pragma unroll
             for (int j4 = 0; j4 < NC; j4 += 4) {
@@ -735,9 +736,6 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
             if (kg == 0) {
                 ldsM[wave][c] = top;
             }
-            if (BF16 && threadIdx.x == 0) {
-                ldsFar = 0;
-            }
             __syncthreads();
             float joint = -INFINITY;
 #pragma unroll
@@ -775,12 +773,20 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
                         o += *reinterpret_cast<const f32x4 *>(sums + (w * L::JOIN_COLS + n - n0) * L::PITCH + d);
                         l += ldsL[w][n];
                     }
+                    bool store = true;
                     if constexpr (BF16) {
-                        if (!(fabsf(o[0]) < FAR) || !(fabsf(o[1]) < FAR) || !(fabsf(o[2]) < FAR) || !(fabsf(o[3]) < FAR)) {
-                            ldsFar = 1;
+                        if (down == 0.0f) { // (the D / 4 lanes of a column agree)
+                            const uint64_t far = __ballot(!(fabsf(o[0]) < FAR) || !(fabsf(o[1]) < FAR) || !(fabsf(o[2]) < FAR) ||
+                                                          !(fabsf(o[3]) < FAR));
+                            constexpr uint64_t COLUMN = D == 256 ? ~0ull : (1ull << (D / 4 % 64)) - 1;
+                            store = ((far >> (lane & ~(D / 4 - 1))) & COLUMN) == 0;
+                            ldsFar[n] = !store;
+                        } else {
+                            store = ldsFar[n];
                         }
                     }
-                    if (whole) {
+                    if (!store) {
+                    } else if (whole) {
                         const float inv = l > 0.0f ? 1.0f / l : (l == l ? 0.0f : l); // nothing seen: zeros; NaN stays
                         const int cc = ct * HT + n;
                         uint16_t *dst = a.out + ((static_cast<int64_t>(seq) * a.tokens + cc / a.group) * a.H + g * a.group + cc % a.group) * D + d;
@@ -797,7 +803,7 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
                                 m = fmaxf(m, ldsM[w][n]);
                             }
                             a.partL[part * HT + n] = l;
-                            a.partM[part * HT + n] = m + (BF16 ? down : 0.0f);
+                            a.partM[part * HT + n] = m;
                         }
                     }
                 }
@@ -806,7 +812,7 @@ __global__ __launch_bounds__(PA_THREADS, D == 256 ? 1 : 2) void PaInt4Kernel(con
             // (stores are counted with loads: the next sequence's tiles are waited for by the number behind them)
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             if constexpr (BF16) {
-                if (down == 0.0f && __builtin_amdgcn_readfirstlane(ldsFar) != 0) { // (what was stored is stored anew)
+                if (down == 0.0f && __ballot(lane < liveCols && ldsFar[lane & (HT - 1)]) != 0) {
                     down = DOWN;
                     continue;
                 }

@@ -95,7 +95,7 @@ def paged_attention_int4(query, key_cache, value_cache, key_params, value_params
     """Attention of query [batch * query_tokens, heads, head_dim] over a 4-bit cache; query token j of a sequence sees its
     first context_lens[b] - query_tokens + 1 + j positions. mask, in the query's type and [batch | 1, heads | 1,
     query_tokens | 1, positions] with positions next to each other, is added to the scaled scores; positions past its
-    length are hidden. `workspace`: a uint8 tensor to use instead of a new one. Tables that reach much further than the
+    length are hidden. `out` may be the query. `workspace`: a uint8 tensor to use instead of a new one. Tables that reach much further than the
     contexts cost short ones a few microseconds (see AtbmiPaInt4Call)."""
     got = (_module or _ext()).paged_attention_int4(query, key_cache, value_cache, key_params, value_params, block_tables,
                                                    context_lens, qk_scale, query_tokens, mask, out, workspace)

@@ -737,7 +737,7 @@ int atbmi_paged_cache_load_int4(const uint8_t *keyCacheDevice, const uint8_t *va
  * Positions in blocks outside [0, numBlocks) are not seen. With a mask (dtype), mask[b * maskSeqStride + h *
  * maskHeadStride + j * maskRowStride + p] (elements; 0: shared) is added to the scaled score; -inf hides the position
  * whatever its score is, and positions at or past maskLen are hidden too. A row that sees nothing is written as zeros.
- * query and out start on 16-byte boundaries. Scores, softmax and sums are fp32; the weights that meet the value codes are
+ * query and out start on 16-byte boundaries; out may be the query itself. Scores, softmax and sums are fp32; the weights that meet the value codes are
  * rounded to bf16 for bf16 models and to twice its bits for fp16 models.
  * maxBlocksPerSeq tells how long a context may be, since the lengths stay on the device: where it allows only short ones
  * (up to 1024 positions, or 2048 with a workgroup for every CU) a workgroup takes whole sequences, else they are cut and a

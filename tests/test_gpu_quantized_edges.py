@@ -207,3 +207,23 @@ def test_load_from_positions_in_front_of_the_first(ops, dev, d, dtype):
                     want[at + t] = full[48 * b + starts[b] + t]
             at += lens[b]
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("values", ["ordinary", "largest", "NaN"])
+@pytest.mark.parametrize("lens,heads,kv_heads,d,block,tokens,cut", LARGE + [([300, 40], 20, 1, 128, 16, 2, False)])
+def test_attention_in_the_place_of_its_query(ops, dev, lens, heads, kv_heads, d, block, tokens, cut, values):
+    """`out` may be the query: the same bits as into another tensor, where sums leave fp32 or a column is NaN as well."""
+    gen = _gen(sum(lens) + d)
+    query, cache, tables, n, scale = _attention_case(ops, dev, gen, lens, heads, kv_heads, d, block, torch.bfloat16, tokens)
+    if cut:
+        tables = _wide(tables, block)
+    own = tables[1][: -(-lens[1] // block)].long().to(dev)
+    if values == "largest":
+        cache[3][own] *= 2.0 ** 124
+    elif values == "NaN":
+        query[tokens, 0, 3] = math.nan
+        cache[3][own[:1], 0, :1] = math.nan
+    query, tables, n = query.to(dev), tables.to(dev), n.to(dev)
+    want = ops.paged_attention_int4(query, *cache, tables, n, scale, query_tokens=tokens)
+    got = ops.paged_attention_int4(query, *cache, tables, n, scale, query_tokens=tokens, out=query)
+    assert got is query and torch.equal(got.view(torch.int16), want.view(torch.int16))
