@@ -725,8 +725,8 @@ struct Plan {
 //   256 x 256   5 + 0.0137 kPer     (32 x 32 tiles of 8192, four rounds: 459; 24 x 8 tiles of 4096, one round: 62)
 //   128 x 128   3 + 0.0061 kPer     (48 x 4 tiles of 4096, one round: 28; 48 x 16, three rounds: 78)
 //   few tokens  2.5 + rounds kPer x {0.0011, 0.0013, 0.0014} (one channel tile and 16, 32, 64 tokens),
-//               {0.0013, 0.0015, 0.0019} (two)   (64 x 6144 x 4096, one round: 11; 64 x 10240 x 8192, a round and a
-//               quarter that counts as two, 34: 25; all with weights from HBM)
+//               {0.0013, 0.0015, 0.0019} (two)   (64 x 6144 x 4096, one round: 11; 64 x 10240 x 8192, two: 33, for
+//               which 128 x 128 tiles in three parts, 25, are taken; all with weights from HBM)
 // and splitting the contraction 4 us and 0.2 a part for the kernel that joins the parts and their bytes at 4 TB/s (128 x 6144 x 4096:
 // 29 whole, 18 in four parts; 512 x 6144 x 4096: 28 whole, 43 in two).
 Plan PlanOf(int64_t m, int64_t n, int64_t k)
